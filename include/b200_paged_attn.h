@@ -352,6 +352,102 @@ B200_API int b200_paged_prefill(const void* q, int64_t q_token_stride,
  * results). No counterpart in the reference (FlashInfer keeps its own). */
 B200_API int64_t b200_paged_prefill_workspace_bytes(void);
 
+/*
+ * Paged KV cache held in 4 bits. No counterpart in the reference, whose
+ * contract accepts only 16-bit caches (attention_backend.py:516-519).
+ *
+ * A row is the head_dim = 128 values of one (slot, KV head) of K or V, in four
+ * groups of 32 along head_dim. Per group, with a = max |x|:
+ *   s = bf16(a / 7) rounded to nearest even (float16 rows: at most 9344, so
+ *       that 7 s is finite in float16); 0 where that is below 2^-126; NaN where
+ *       a is not finite
+ *   c = 8 + rint(x * (1 / s)), the reciprocal and the product each rounded to
+ *       fp32 once, half to even (8 where s is 0 or NaN)
+ * and each value stands for s * (c - 8): a group with an infinity or a NaN
+ * reads back as NaN. 64 bytes of codes (element 2i in the low nibble of byte
+ * i) and 8 bytes of scales make a row of B200_INT4_ROW_BYTES.
+ *
+ * A page of block_size slots holds, per tensor, first all codes, then all
+ * scales, both head-major:
+ *   codes  [num_kv_heads][block_size][64] bytes
+ *   scales [num_kv_heads][block_size][4] bf16
+ */
+#define B200_INT4_GROUP 32
+#define B200_INT4_ROW_BYTES 72
+typedef struct b200_int4_cache {
+  void* k_cache; /* 16-byte aligned; written only by b200_store_kvcache_int4 */
+  void* v_cache;
+  int64_t num_blocks;
+  int32_t block_size;   /* multiple of 16 */
+  int32_t num_kv_heads;
+  int64_t block_stride_bytes; /* >= block_size * num_kv_heads * 72, multiple of 16 */
+} b200_int4_cache;
+
+/*
+ * KV append into a 4-bit cache: every token i with slot s != -1 quantises its
+ * num_kv_heads rows of 128 `dtype` values at key + i * key_row_stride into
+ * slot s of k_cache, and the value row into v_cache. Slots outside
+ * [0, num_blocks * block_size) other than -1 are skipped and reported as
+ * B200_STATUS_SLOT_OUT_OF_RANGE. A slot named twice in one call holds an
+ * unspecified mixture of its rows. Rows 16-byte aligned, row strides multiples
+ * of 8 elements and at least num_kv_heads * 128.
+ */
+B200_API int b200_store_kvcache_int4(const void* key, int64_t key_row_stride,
+                                     const void* value, int64_t value_row_stride,
+                                     int32_t dtype, const b200_int4_cache* cache,
+                                     const void* slot_mapping, int32_t slot_is_int64,
+                                     int64_t num_tokens, int32_t* status, void* stream);
+
+/*
+ * The way back: row i of key / value (num_kv_heads * 128 values of `dtype`)
+ * receives slot slot_mapping[i]'s values s * (c - 8), rounded to `dtype` once
+ * (past float16's range: infinity; rows stored from float16 never are). Slots
+ * of -1 leave their row as it was, slots out of range too, with a report.
+ */
+B200_API int b200_load_kvcache_int4(const b200_int4_cache* cache, const void* slot_mapping,
+                                    int32_t slot_is_int64, int64_t num_tokens, void* key,
+                                    int64_t key_row_stride, void* value,
+                                    int64_t value_row_stride, int32_t dtype,
+                                    int32_t* status, void* stream);
+
+/* b200_paged_decode_plan for a 4-bit cache (head_dim 128). */
+B200_API int b200_paged_decode_int4_plan(int32_t num_seqs, int32_t num_q_heads,
+                                         int32_t num_kv_heads, int32_t block_size,
+                                         int32_t max_kv_len, int64_t total_kv_tokens,
+                                         int32_t force_num_parts, b200_decode_plan* plan);
+
+/*
+ * b200_paged_decode over a 4-bit cache; q and out are `dtype`. max_blocks is
+ * the number of valid columns of block_tables: a token past them, or a page id
+ * outside the pool, counts as a row of zeros and sets
+ * B200_STATUS_PAGE_OUT_OF_RANGE. A sequence of length 0 gives zeros. The kernel
+ * is a programmatic dependent of the kernel before it on `stream`, as
+ * b200_paged_decode is, but reads nothing before that kernel has completed.
+ */
+B200_API int b200_paged_decode_int4(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                                    int32_t dtype, const b200_int4_cache* cache,
+                                    const int32_t* block_tables, int64_t block_table_stride,
+                                    int32_t max_blocks, const int32_t* seq_lens,
+                                    int32_t num_seqs, int32_t num_q_heads, void* out,
+                                    int64_t out_seq_stride, int64_t out_head_stride,
+                                    float softmax_scale, const b200_decode_plan* plan,
+                                    void* workspace, int64_t workspace_bytes, int32_t* status,
+                                    void* stream);
+
+/*
+ * b200_paged_prefill over a 4-bit cache; q and out are `dtype`, max_blocks as
+ * above. softmax_scale must be positive. No workspace.
+ */
+B200_API int b200_paged_prefill_int4(const void* q, int64_t q_token_stride,
+                                     int64_t q_head_stride, int32_t dtype,
+                                     const b200_int4_cache* cache, const int32_t* block_tables,
+                                     int64_t block_table_stride, int32_t max_blocks,
+                                     const int32_t* seq_lens, const int32_t* query_start_loc,
+                                     int32_t num_seqs, int32_t num_q_tokens, int32_t max_q_len,
+                                     int32_t num_q_heads, void* out, int64_t out_token_stride,
+                                     int64_t out_head_stride, float softmax_scale,
+                                     int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

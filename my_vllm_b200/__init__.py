@@ -2,7 +2,7 @@
 
 Three hand-written CUDA kernels behind a C ABI (``include/b200_paged_attn.h``):
 the KV-cache append, paged GQA decode (flash-decoding with split-KV) and paged
-chunked prefill. ``B200PagedBackend`` serves them through the engine's
+chunked prefill, over 16-bit, FP8 and 4-bit caches. ``B200PagedBackend`` serves them through the engine's
 ``AttentionBackend`` contract; ``kv_store.install()`` routes the engine's KV
 append to the B200 kernel.
 
@@ -10,7 +10,16 @@ append to the B200 kernel.
 names below need the engine (``nanovllm``) and are imported on first use.
 """
 
-from .ops import DecodePlan, paged_decode, paged_prefill, plan_decode, store_kvcache
+from .ops import (
+    DecodePlan,
+    int4_cache_shape,
+    load_kvcache_int4,
+    paged_decode,
+    paged_prefill,
+    plan_decode,
+    store_kvcache,
+    store_kvcache_int4,
+)
 
 _BACKEND_NAMES = ("B200PagedBackend", "B200PagedMetadata", "register")
 
@@ -27,9 +36,12 @@ __all__ = [
     "B200PagedBackend",
     "B200PagedMetadata",
     "DecodePlan",
+    "int4_cache_shape",
+    "load_kvcache_int4",
     "paged_decode",
     "paged_prefill",
     "plan_decode",
     "register",
     "store_kvcache",
+    "store_kvcache_int4",
 ]

@@ -29,7 +29,10 @@ DTYPE_FLOAT16 = 0
 DTYPE_BFLOAT16 = 1
 DTYPE_FP8_E4M3 = 2
 
-ABI_VERSION = 300
+ABI_VERSION = 301
+
+# Bytes of one 4-bit cache row of 128 values (B200_INT4_ROW_BYTES).
+INT4_ROW_BYTES = 72
 
 # Size of the scratch array built into the library for
 # b200_paged_decode_noalloc (B200_NOALLOC_DECODE_SCRATCH_BYTES).
@@ -50,6 +53,11 @@ EXPORTED_SYMBOLS = (
     "b200_paged_prefill",
     "b200_paged_prefill_workspace_bytes",
     "b200_paged_decode_noalloc",
+    "b200_store_kvcache_int4",
+    "b200_load_kvcache_int4",
+    "b200_paged_decode_int4_plan",
+    "b200_paged_decode_int4",
+    "b200_paged_prefill_int4",
 )
 
 
@@ -70,6 +78,19 @@ class PagedCache(ctypes.Structure):
         ("kv_fp8", ctypes.c_int32),
         ("k_scale", ctypes.c_void_p),
         ("v_scale", ctypes.c_void_p),
+    ]
+
+
+class Int4Cache(ctypes.Structure):
+    """Mirror of ``b200_int4_cache``."""
+
+    _fields_ = [
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("num_blocks", ctypes.c_int64),
+        ("block_size", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("block_stride_bytes", ctypes.c_int64),
     ]
 
 
@@ -145,6 +166,32 @@ _SIGNATURES = {
         _I32,
     ),
     "b200_paged_prefill_workspace_bytes": ([], _I64),
+    "b200_store_kvcache_int4": (
+        [_VP, _I64, _VP, _I64, _I32, ctypes.POINTER(Int4Cache), _VP, _I32, _I64, _VP, _VP],
+        _I32,
+    ),
+    "b200_load_kvcache_int4": (
+        [ctypes.POINTER(Int4Cache), _VP, _I32, _I64, _VP, _I64, _VP, _I64, _I32, _VP, _VP],
+        _I32,
+    ),
+    "b200_paged_decode_int4_plan": (
+        [_I32, _I32, _I32, _I32, _I32, _I64, _I32, ctypes.POINTER(DecodePlan)],
+        _I32,
+    ),
+    "b200_paged_decode_int4": (
+        [
+            _VP, _I64, _I64, _I32, ctypes.POINTER(Int4Cache), _VP, _I64, _I32, _VP, _I32, _I32,
+            _VP, _I64, _I64, _F32, ctypes.POINTER(DecodePlan), _VP, _I64, _VP, _VP,
+        ],
+        _I32,
+    ),
+    "b200_paged_prefill_int4": (
+        [
+            _VP, _I64, _I64, _I32, ctypes.POINTER(Int4Cache), _VP, _I64, _I32, _VP, _VP, _I32,
+            _I32, _I32, _I32, _VP, _I64, _I64, _F32, _VP, _VP,
+        ],
+        _I32,
+    ),
 }
 
 _lock = threading.Lock()
@@ -185,7 +232,8 @@ _torch_ops_loaded = False
 
 def load_torch_ops():
     """Register the ``torch.ops.b200`` operators (kv_append, paged_decode,
-    paged_prefill) from the in-tree operator library; returns ``torch.ops.b200``.
+    paged_prefill and their ``_int4`` forms, kv_load_int4) from the in-tree
+    operator library; returns ``torch.ops.b200``.
     RuntimeError if either library is missing."""
     global _torch_ops_loaded
     import torch

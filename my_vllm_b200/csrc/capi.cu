@@ -15,6 +15,7 @@
 #include <unordered_map>
 
 #include "../../include/b200_paged_attn.h"
+#include "kv_int4.cuh"
 #include "paged_decode.cuh"
 #include "paged_prefill.cuh"
 #include "rope_append.cuh"
@@ -232,7 +233,7 @@ void set_last_error(const std::string& message) { g_last_error = message; }
 
 extern "C" {
 
-int b200_abi_version(void) { return 300; }
+int b200_abi_version(void) { return 301; }
 
 const char* b200_last_error(void) { return g_last_error.c_str(); }
 
@@ -661,6 +662,223 @@ int b200_paged_prefill(const void* q, int64_t q_token_stride, int64_t q_head_str
                                                 cache->num_kv_heads, num_seqs, max_q_len,
                                                 static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "paged prefill launch");
+  return B200_OK;
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------ 4-bit caches --
+namespace {
+
+int validate_int4_cache(const b200_int4_cache* c, b200::Int4Cache* out) {
+  if (c == nullptr) return fail(B200_ERR_INVALID_ARGUMENT, "cache descriptor is NULL");
+  if (c->k_cache == nullptr || c->v_cache == nullptr)
+    return fail(B200_ERR_INVALID_ARGUMENT, "key and value caches must both be present");
+  if (c->block_size <= 0 || c->block_size % b200::kTileTokens != 0)
+    return fail(B200_ERR_UNSUPPORTED, "block_size must be a positive multiple of 16");
+  if (c->num_kv_heads <= 0 || c->num_blocks <= 0)
+    return fail(B200_ERR_INVALID_ARGUMENT, "num_kv_heads and num_blocks must be positive");
+  if (c->num_blocks > (int64_t(1) << 31) - 1 ||
+      (int64_t)c->block_size * c->num_kv_heads > (int64_t(1) << 24))
+    return fail(B200_ERR_UNSUPPORTED, "num_blocks must fit in int32, a page in 2^24 rows");
+  if (((reinterpret_cast<uintptr_t>(c->k_cache) | reinterpret_cast<uintptr_t>(c->v_cache)) & 15) !=
+      0)
+    return fail(B200_ERR_INVALID_ARGUMENT, "cache base pointers must be 16-byte aligned");
+  if (c->block_stride_bytes % 16 ||
+      c->block_stride_bytes < (int64_t)c->block_size * c->num_kv_heads * b200::kInt4RowBytes)
+    return fail(B200_ERR_INVALID_ARGUMENT,
+                "block stride must cover a page and be a multiple of 16 bytes");
+  out->k = static_cast<uint8_t*>(c->k_cache);
+  out->v = static_cast<uint8_t*>(c->v_cache);
+  out->block_stride = c->block_stride_bytes;
+  out->num_blocks = c->num_blocks;
+  out->block_size = c->block_size;
+  out->num_kv_heads = c->num_kv_heads;
+  return B200_OK;
+}
+
+int validate_int4_dtype(int32_t dtype) {
+  if (dtype != B200_DTYPE_BFLOAT16 && dtype != B200_DTYPE_FLOAT16)
+    return fail(B200_ERR_UNSUPPORTED, "dtype must be float16 or bfloat16");
+  return B200_OK;
+}
+
+// The 16-bit rows of the append and the read-back.
+int validate_int4_rows(const void* key, int64_t key_row_stride, const void* value,
+                       int64_t value_row_stride, const void* slots, int64_t num_tokens,
+                       int num_kv_heads) {
+  if (!key || !value || !slots) return fail(B200_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  if (((reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value)) & 15) ||
+      (key_row_stride | value_row_stride) % 8)
+    return fail(B200_ERR_INVALID_ARGUMENT,
+                "rows must be 16-byte aligned with strides that are multiples of 8 elements");
+  const int64_t row = (int64_t)num_kv_heads * b200::kHeadDim;
+  if (num_tokens > 1 && (key_row_stride < row || value_row_stride < row))
+    return fail(B200_ERR_INVALID_ARGUMENT, "row strides must cover all KV heads");
+  return B200_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int b200_store_kvcache_int4(const void* key, int64_t key_row_stride, const void* value,
+                            int64_t value_row_stride, int32_t dtype, const b200_int4_cache* cache,
+                            const void* slot_mapping, int32_t slot_is_int64, int64_t num_tokens,
+                            int32_t* status, void* stream) {
+  g_last_error.clear();
+  b200::Int4Cache c;
+  int rc = validate_int4_dtype(dtype);
+  if (rc == B200_OK) rc = validate_int4_cache(cache, &c);
+  if (rc != B200_OK) return rc;
+  if (num_tokens < 0) return fail(B200_ERR_INVALID_ARGUMENT, "num_tokens must be >= 0");
+  if (num_tokens == 0) return B200_OK;
+  rc = validate_int4_rows(key, key_row_stride, value, value_row_stride, slot_mapping, num_tokens,
+                          c.num_kv_heads);
+  if (rc != B200_OK) return rc;
+  cudaError_t e = b200::launch_store_kvcache_int4(key, key_row_stride, value, value_row_stride,
+                                                  dtype, c, slot_mapping, slot_is_int64 != 0,
+                                                  num_tokens, status,
+                                                  static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "int4 KV append launch");
+  return B200_OK;
+}
+
+int b200_load_kvcache_int4(const b200_int4_cache* cache, const void* slot_mapping,
+                           int32_t slot_is_int64, int64_t num_tokens, void* key,
+                           int64_t key_row_stride, void* value, int64_t value_row_stride,
+                           int32_t dtype, int32_t* status, void* stream) {
+  g_last_error.clear();
+  b200::Int4Cache c;
+  int rc = validate_int4_dtype(dtype);
+  if (rc == B200_OK) rc = validate_int4_cache(cache, &c);
+  if (rc != B200_OK) return rc;
+  if (num_tokens < 0) return fail(B200_ERR_INVALID_ARGUMENT, "num_tokens must be >= 0");
+  if (num_tokens == 0) return B200_OK;
+  rc = validate_int4_rows(key, key_row_stride, value, value_row_stride, slot_mapping, num_tokens,
+                          c.num_kv_heads);
+  if (rc != B200_OK) return rc;
+  cudaError_t e = b200::launch_load_kvcache_int4(c, slot_mapping, slot_is_int64 != 0, num_tokens,
+                                                 key, key_row_stride, value, value_row_stride,
+                                                 dtype, status, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "int4 KV read-back launch");
+  return B200_OK;
+}
+
+int b200_paged_decode_int4_plan(int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
+                                int32_t block_size, int32_t max_kv_len, int64_t total_kv_tokens,
+                                int32_t force_num_parts, b200_decode_plan* plan) {
+  return b200_paged_decode_plan(num_seqs, num_q_heads, num_kv_heads, b200::kHeadDim, block_size,
+                                max_kv_len, total_kv_tokens, force_num_parts, 1, plan);
+}
+
+int b200_paged_decode_int4(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                           int32_t dtype, const b200_int4_cache* cache,
+                           const int32_t* block_tables, int64_t block_table_stride,
+                           int32_t max_blocks, const int32_t* seq_lens, int32_t num_seqs,
+                           int32_t num_q_heads, void* out, int64_t out_seq_stride,
+                           int64_t out_head_stride, float softmax_scale,
+                           const b200_decode_plan* plan, void* workspace,
+                           int64_t workspace_bytes, int32_t* status, void* stream) {
+  g_last_error.clear();
+  b200::Int4Cache c;
+  int rc = validate_int4_dtype(dtype);
+  if (rc == B200_OK) rc = validate_int4_cache(cache, &c);
+  if (rc != B200_OK) return rc;
+  if (plan == nullptr) return fail(B200_ERR_INVALID_ARGUMENT, "plan is NULL");
+  if (num_seqs < 0 || max_blocks < 0)
+    return fail(B200_ERR_INVALID_ARGUMENT, "num_seqs and max_blocks must be >= 0");
+  if (num_q_heads <= 0 || num_q_heads % c.num_kv_heads)
+    return fail(B200_ERR_INVALID_ARGUMENT, "num_q_heads must be divisible by num_kv_heads");
+  const int group = num_q_heads / c.num_kv_heads;
+  if (group > 16) return fail(B200_ERR_UNSUPPORTED, "at most 16 q heads per KV head");
+  if (plan->num_parts < 1 || plan->part_tokens <= 0 || plan->part_tokens % b200::kTileTokens ||
+      plan->part_tokens > b200::kMaxPartTokens)
+    return fail(B200_ERR_INVALID_ARGUMENT, "malformed decode plan");
+  if (num_seqs == 0) return B200_OK;
+  if (!q || !out || !block_tables || !seq_lens)
+    return fail(B200_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 3) ||
+      (q_seq_stride | q_head_stride | out_seq_stride | out_head_stride) & 1)
+    return fail(B200_ERR_INVALID_ARGUMENT, "q/out must be 4-byte aligned with even strides");
+  const int64_t need = decode_workspace_bytes(num_seqs, num_q_heads, plan->num_parts);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(B200_ERR_INVALID_ARGUMENT,
+                "decode workspace too small: need " + std::to_string(need) + " bytes");
+  if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return fail(B200_ERR_INVALID_ARGUMENT, "decode workspace must be 256-byte aligned");
+  b200::Int4AttnParams p{};
+  p.q = q;
+  p.q_token_stride = q_seq_stride;
+  p.q_head_stride = q_head_stride;
+  p.block_tables = block_tables;
+  p.block_table_stride = block_table_stride;
+  p.max_blocks = max_blocks;
+  p.seq_lens = seq_lens;
+  p.plan_tokens = (int64_t)plan->num_parts * plan->part_tokens;
+  p.out = out;
+  p.out_token_stride = out_seq_stride;
+  p.out_head_stride = out_head_stride;
+  p.num_seqs = num_seqs;
+  p.num_q_tokens = num_seqs;
+  p.num_q_heads = num_q_heads;
+  p.group = group;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.status = status;
+  cudaError_t e = b200::launch_int4_attention(c, p, dtype, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "int4 paged decode launch");
+  return B200_OK;
+}
+
+int b200_paged_prefill_int4(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                            int32_t dtype, const b200_int4_cache* cache,
+                            const int32_t* block_tables, int64_t block_table_stride,
+                            int32_t max_blocks, const int32_t* seq_lens,
+                            const int32_t* query_start_loc, int32_t num_seqs,
+                            int32_t num_q_tokens, int32_t max_q_len, int32_t num_q_heads,
+                            void* out, int64_t out_token_stride, int64_t out_head_stride,
+                            float softmax_scale, int32_t* status, void* stream) {
+  g_last_error.clear();
+  b200::Int4Cache c;
+  int rc = validate_int4_dtype(dtype);
+  if (rc == B200_OK) rc = validate_int4_cache(cache, &c);
+  if (rc != B200_OK) return rc;
+  if (num_seqs < 0 || num_q_tokens < 0 || max_q_len < 0 || max_blocks < 0)
+    return fail(B200_ERR_INVALID_ARGUMENT, "sizes must be >= 0");
+  if (num_q_heads <= 0 || num_q_heads % c.num_kv_heads)
+    return fail(B200_ERR_INVALID_ARGUMENT, "num_q_heads must be divisible by num_kv_heads");
+  const int group = num_q_heads / c.num_kv_heads;
+  if (group > 128) return fail(B200_ERR_UNSUPPORTED, "at most 128 q heads per KV head");
+  if (!(softmax_scale > 0.f))
+    return fail(B200_ERR_INVALID_ARGUMENT, "softmax_scale must be positive");
+  if (num_seqs == 0 || num_q_tokens == 0) return B200_OK;
+  if (!q || !out || !block_tables || !seq_lens || !query_start_loc)
+    return fail(B200_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
+  if (max_q_len <= 0) return fail(B200_ERR_INVALID_ARGUMENT, "max_q_len must be positive");
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) ||
+      (q_token_stride | q_head_stride | out_token_stride | out_head_stride) & 7)
+    return fail(B200_ERR_INVALID_ARGUMENT,
+                "q/out must be 16-byte aligned with strides that are multiples of 8");
+  b200::Int4AttnParams p{};
+  p.q = q;
+  p.q_token_stride = q_token_stride;
+  p.q_head_stride = q_head_stride;
+  p.block_tables = block_tables;
+  p.block_table_stride = block_table_stride;
+  p.max_blocks = max_blocks;
+  p.seq_lens = seq_lens;
+  p.query_start_loc = query_start_loc;
+  p.out = out;
+  p.out_token_stride = out_token_stride;
+  p.out_head_stride = out_head_stride;
+  p.num_seqs = num_seqs;
+  p.num_q_tokens = num_q_tokens;
+  p.num_q_heads = num_q_heads;
+  p.group = group;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.status = status;
+  cudaError_t e = b200::launch_int4_attention(c, p, dtype, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "int4 paged prefill launch");
   return B200_OK;
 }
 

@@ -1,0 +1,76 @@
+// kv_int4.cuh — the 4-bit KV cache: row format, page layout and the launch
+// functions of the kernels that write it, read it back and attend over it.
+//
+// A row is the 128 values of one (slot, KV head) of K or V in four groups of
+// 32 along head_dim. Per group, with a = max |x|:
+//   s = bf16(a / 7) (nearest even; fp16 rows at most 9344, so 7 s is finite in
+//       fp16), 0 below 2^-126, NaN where a is not finite
+//   c = 8 + rne(fl32(x * fl32(1 / s))), 1..15 (8 where s is 0 or NaN)
+// and the group stands for s * (c - 8). A row takes 64 bytes of codes (even
+// elements in the low nibble) and 8 bytes of scales: 4.5 bits per value.
+//
+// A page of block_size slots holds, per tensor, all codes and then all scales,
+// both head-major:
+//   codes  [num_kv_heads][block_size][64 bytes]
+//   scales [num_kv_heads][block_size][4] bf16
+// so that the 16 rows of one (tile, head) are 1 KiB of codes and 128 bytes of
+// scales, each contiguous, whatever the number of heads.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace b200 {
+
+constexpr int kInt4GroupElems = 32;
+constexpr int kInt4CodeBytes = 64;   // of a row
+constexpr int kInt4ScaleBytes = 8;   // of a row
+constexpr int kInt4RowBytes = kInt4CodeBytes + kInt4ScaleBytes;
+
+struct Int4Cache {
+  uint8_t* k;
+  uint8_t* v;
+  int64_t block_stride;  // bytes between consecutive pages
+  int64_t num_blocks;
+  int block_size;
+  int num_kv_heads;
+};
+
+cudaError_t launch_store_kvcache_int4(const void* key, int64_t key_row_stride, const void* value,
+                                      int64_t value_row_stride, int dtype, const Int4Cache& cache,
+                                      const void* slots, bool slot64, int64_t num_tokens,
+                                      int32_t* status, cudaStream_t stream);
+
+cudaError_t launch_load_kvcache_int4(const Int4Cache& cache, const void* slots, bool slot64,
+                                     int64_t num_tokens, void* key, int64_t key_row_stride,
+                                     void* value, int64_t value_row_stride, int dtype,
+                                     int32_t* status, cudaStream_t stream);
+
+// Attention over a 4-bit cache. Decode: one query row per sequence
+// (query_start_loc NULL); prefill: rows [query_start_loc[s], query_start_loc[s+1]).
+struct Int4AttnParams {
+  const void* q;
+  int64_t q_token_stride;
+  int64_t q_head_stride;
+  const int32_t* block_tables;
+  int64_t block_table_stride;
+  int max_blocks;  // valid columns of a block-table row
+  const int32_t* seq_lens;
+  const int32_t* query_start_loc;
+  int64_t plan_tokens;  // decode: what the plan covers of each sequence
+  void* out;
+  int64_t out_token_stride;
+  int64_t out_head_stride;
+  int num_seqs;
+  int num_q_tokens;
+  int num_q_heads;
+  int group;  // q heads per KV head
+  float scale_log2;  // softmax_scale * log2(e)
+  int32_t* status;
+};
+
+cudaError_t launch_int4_attention(const Int4Cache& cache, const Int4AttnParams& p, int dtype,
+                                  cudaStream_t stream);
+
+}  // namespace b200

@@ -12,10 +12,17 @@
 //   kv_append      <- store_kvcache (nanovllm/layers/attention.py:34-41)
 //   paged_decode   <- BatchDecodeWithPagedKVCacheWrapper.run (attention_backend.py:995-997)
 //   paged_prefill  <- BatchPrefillWithPagedKVCacheWrapper.run (attention_backend.py:992-994)
+//
+// kv_append_int4, kv_load_int4, paged_decode_int4 and paged_prefill_int4 are the
+// same over 4-bit caches (uint8 [num_blocks, block_size, num_kv_heads, 72]); they
+// also check that every tensor is on one device and make it current.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <functional>
+#include <initializer_list>
 #include <optional>
 
 #include "../../include/b200_paged_attn.h"
@@ -241,7 +248,187 @@ void paged_prefill(const at::Tensor& q, const at::Tensor& k_cache, const at::Ten
             "b200_paged_prefill");
 }
 
+// ------------------------------------------------------------ 4-bit caches --
+// The cache pair uint8 [num_blocks, block_size, num_kv_heads, 72]; pages may be
+// strided, the inside of a page is packed.
+b200_int4_cache int4_cache_desc(const at::Tensor& k, const at::Tensor& v) {
+  require_cuda(k, "k_cache");
+  require_cuda(v, "v_cache");
+  TORCH_CHECK(k.scalar_type() == at::kByte && v.scalar_type() == at::kByte,
+              "b200: 4-bit caches must be uint8");
+  TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes() && k.size(3) == B200_INT4_ROW_BYTES,
+              "b200: 4-bit caches must have shape [pages, block_size, num_kv_heads, 72]");
+  TORCH_CHECK(k.strides() == v.strides(), "b200: key and value caches must have identical strides");
+  TORCH_CHECK(k.stride(3) == 1 && k.stride(2) == B200_INT4_ROW_BYTES &&
+                  k.stride(1) == k.size(2) * B200_INT4_ROW_BYTES,
+              "b200: the pages of a 4-bit cache must be packed");
+  TORCH_CHECK(k.size(1) <= INT32_MAX && k.size(2) <= INT32_MAX, "b200: cache too large");
+  b200_int4_cache c{};
+  c.k_cache = k.data_ptr();
+  c.v_cache = v.data_ptr();
+  c.num_blocks = k.size(0);
+  c.block_size = static_cast<int32_t>(k.size(1));
+  c.num_kv_heads = static_cast<int32_t>(k.size(2));
+  // the stride of a size-1 dimension carries no layout
+  c.block_stride_bytes = k.size(0) == 1 ? k.size(1) * k.stride(1) : k.stride(0);
+  return c;
+}
+
+void same_device(const at::Tensor& first,
+                 std::initializer_list<std::reference_wrapper<const at::Tensor>> rest,
+                 std::initializer_list<std::reference_wrapper<const std::optional<at::Tensor>>> opt) {
+  for (const at::Tensor& t : rest)
+    TORCH_CHECK(t.device() == first.device(), "b200: every tensor must be on one device");
+  for (const std::optional<at::Tensor>& t : opt)
+    TORCH_CHECK(!t.has_value() || t->device() == first.device(),
+                "b200: every tensor must be on one device");
+}
+
+// The 16-bit rows [tokens, num_kv_heads, 128] of the append and the read-back.
+void require_int4_rows(const at::Tensor& key, const at::Tensor& value, const at::Tensor& cache,
+                       const at::Tensor& slots) {
+  TORCH_CHECK(key.dim() == 3 && key.sizes() == value.sizes() && key.size(1) == cache.size(2) &&
+                  key.size(2) == 128 && key.scalar_type() == value.scalar_type(),
+              "b200: key and value must be [tokens, num_kv_heads, 128] of one type");
+  TORCH_CHECK(key.stride(2) == 1 && value.stride(2) == 1 &&
+                  (key.size(1) == 1 || (key.stride(1) == 128 && value.stride(1) == 128)),
+              "b200: key/value heads must be packed (stride(1) == head_dim)");
+  require_cuda(slots, "slot_mapping");
+  TORCH_CHECK(slots.scalar_type() == at::kInt || slots.scalar_type() == at::kLong,
+              "b200: slot_mapping must be int32 or int64");
+  TORCH_CHECK(slots.dim() == 1 && slots.numel() == key.size(0) &&
+                  (slots.numel() <= 1 || slots.stride(0) == 1),
+              "b200: slot_mapping must be a contiguous 1-D tensor of one slot per token");
+}
+
+// Rows of a single token have no stride of their own.
+int64_t row_stride(const at::Tensor& t) {
+  return t.size(0) <= 1 ? t.size(1) * t.size(2) : t.stride(0);
+}
+
+void kv_append_int4(const at::Tensor& key, const at::Tensor& value, at::Tensor& k_cache,
+                    at::Tensor& v_cache, const at::Tensor& slot_mapping,
+                    const std::optional<at::Tensor>& status) {
+  require_cuda(key, "key");
+  require_cuda(value, "value");
+  const b200_int4_cache cache = int4_cache_desc(k_cache, v_cache);
+  require_int4_rows(key, value, k_cache, slot_mapping);
+  same_device(key, {value, k_cache, v_cache, slot_mapping}, {status});
+  const c10::cuda::CUDAGuard guard(key.device());
+  check_abi(b200_store_kvcache_int4(key.data_ptr(), row_stride(key), value.data_ptr(),
+                                    row_stride(value), activation_dtype(key.scalar_type()), &cache,
+                                    slot_mapping.data_ptr(),
+                                    slot_mapping.scalar_type() == at::kLong ? 1 : 0, key.size(0),
+                                    status_ptr(status), current_stream(key)),
+            "b200_store_kvcache_int4");
+}
+
+void kv_load_int4(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                  const at::Tensor& slot_mapping, at::Tensor& key, at::Tensor& value,
+                  const std::optional<at::Tensor>& status) {
+  require_cuda(key, "key");
+  require_cuda(value, "value");
+  const b200_int4_cache cache = int4_cache_desc(k_cache, v_cache);
+  require_int4_rows(key, value, k_cache, slot_mapping);
+  same_device(key, {value, k_cache, v_cache, slot_mapping}, {status});
+  const c10::cuda::CUDAGuard guard(key.device());
+  check_abi(b200_load_kvcache_int4(&cache, slot_mapping.data_ptr(),
+                                   slot_mapping.scalar_type() == at::kLong ? 1 : 0, key.size(0),
+                                   key.data_ptr(), row_stride(key), value.data_ptr(),
+                                   row_stride(value), activation_dtype(key.scalar_type()),
+                                   status_ptr(status), current_stream(key)),
+            "b200_load_kvcache_int4");
+}
+
+void require_attention(const at::Tensor& q, const at::Tensor& out, const at::Tensor& block_tables,
+                       const at::Tensor& seq_lens) {
+  require_cuda(q, "q");
+  require_cuda(out, "out");
+  TORCH_CHECK(q.dim() == 3 && out.sizes() == q.sizes() && q.size(2) == 128 && q.stride(2) == 1 &&
+                  out.stride(2) == 1,
+              "b200: q and out must be [tokens, num_q_heads, 128], head_dim contiguous");
+  TORCH_CHECK(out.scalar_type() == q.scalar_type(), "b200: out must have the query dtype");
+  require_block_tables(block_tables);
+  require_int32_vector(seq_lens, "seq_lens");
+}
+
+void paged_decode_int4(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                       const at::Tensor& block_tables, const at::Tensor& seq_lens, at::Tensor& out,
+                       int64_t num_parts, int64_t part_tokens, double softmax_scale,
+                       const std::optional<at::Tensor>& workspace,
+                       const std::optional<at::Tensor>& status) {
+  require_attention(q, out, block_tables, seq_lens);
+  const int64_t b = q.size(0);
+  TORCH_CHECK(block_tables.size(0) >= b && seq_lens.numel() >= b,
+              "b200: block_tables / seq_lens must have one row per sequence");
+  TORCH_CHECK(num_parts <= INT32_MAX && part_tokens <= INT32_MAX, "b200: malformed decode plan");
+  const b200_int4_cache cache = int4_cache_desc(k_cache, v_cache);
+  same_device(q, {k_cache, v_cache, block_tables, seq_lens, out}, {workspace, status});
+  void* ws = nullptr;
+  int64_t ws_bytes = 0;
+  if (workspace.has_value()) {
+    TORCH_CHECK(workspace->is_contiguous(), "b200: workspace must be contiguous");
+    ws = workspace->data_ptr();
+    ws_bytes = workspace->numel() * workspace->element_size();
+  }
+  b200_decode_plan plan{static_cast<int32_t>(num_parts), static_cast<int32_t>(part_tokens), 0};
+  const c10::cuda::CUDAGuard guard(q.device());
+  check_abi(b200_paged_decode_int4(q.data_ptr(), q.stride(0), q.stride(1),
+                                   activation_dtype(q.scalar_type()), &cache,
+                                   block_tables.data_ptr<int32_t>(), block_tables.stride(0),
+                                   static_cast<int32_t>(block_tables.size(1)),
+                                   seq_lens.data_ptr<int32_t>(), static_cast<int32_t>(b),
+                                   static_cast<int32_t>(q.size(1)), out.data_ptr(), out.stride(0),
+                                   out.stride(1), static_cast<float>(softmax_scale), &plan, ws,
+                                   ws_bytes, status_ptr(status), current_stream(q)),
+            "b200_paged_decode_int4");
+}
+
+void paged_prefill_int4(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                        const at::Tensor& block_tables, const at::Tensor& seq_lens,
+                        const at::Tensor& query_start_loc, at::Tensor& out, int64_t max_q_len,
+                        double softmax_scale, int64_t num_seqs,
+                        const std::optional<at::Tensor>& status) {
+  require_attention(q, out, block_tables, seq_lens);
+  require_int32_vector(query_start_loc, "query_start_loc");
+  TORCH_CHECK(num_seqs >= 0 && query_start_loc.numel() >= num_seqs + 1 &&
+                  block_tables.size(0) >= num_seqs && seq_lens.numel() >= num_seqs,
+              "b200: query_start_loc / block_tables / seq_lens too short for num_seqs");
+  TORCH_CHECK(max_q_len <= INT32_MAX && q.size(0) <= INT32_MAX, "b200: too many query rows");
+  const b200_int4_cache cache = int4_cache_desc(k_cache, v_cache);
+  same_device(q, {k_cache, v_cache, block_tables, seq_lens, query_start_loc, out}, {status});
+  const c10::cuda::CUDAGuard guard(q.device());
+  check_abi(b200_paged_prefill_int4(q.data_ptr(), q.stride(0), q.stride(1),
+                                    activation_dtype(q.scalar_type()), &cache,
+                                    block_tables.data_ptr<int32_t>(), block_tables.stride(0),
+                                    static_cast<int32_t>(block_tables.size(1)),
+                                    seq_lens.data_ptr<int32_t>(),
+                                    query_start_loc.data_ptr<int32_t>(),
+                                    static_cast<int32_t>(num_seqs),
+                                    static_cast<int32_t>(q.size(0)),
+                                    static_cast<int32_t>(max_q_len),
+                                    static_cast<int32_t>(q.size(1)), out.data_ptr(), out.stride(0),
+                                    out.stride(1), static_cast<float>(softmax_scale),
+                                    status_ptr(status), current_stream(q)),
+            "b200_paged_prefill_int4");
+}
+
 // ------------------------------------------------ Meta (FakeTensor) kernels --
+void kv_append_int4_meta(const at::Tensor&, const at::Tensor&, at::Tensor&, at::Tensor&,
+                         const at::Tensor&, const std::optional<at::Tensor>&) {}
+
+void kv_load_int4_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, at::Tensor&,
+                       at::Tensor&, const std::optional<at::Tensor>&) {}
+
+void paged_decode_int4_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                            const at::Tensor&, const at::Tensor&, at::Tensor&, int64_t, int64_t,
+                            double, const std::optional<at::Tensor>&,
+                            const std::optional<at::Tensor>&) {}
+
+void paged_prefill_int4_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                             const at::Tensor&, const at::Tensor&, const at::Tensor&, at::Tensor&,
+                             int64_t, double, int64_t, const std::optional<at::Tensor>&) {}
+
 void kv_append_meta(const at::Tensor&, const at::Tensor&, at::Tensor&, at::Tensor&,
                     const at::Tensor&, const std::optional<at::Tensor>&,
                     const std::optional<at::Tensor>&, const std::optional<at::Tensor>&) {}
@@ -275,16 +462,38 @@ TORCH_LIBRARY(b200, m) {
       "Tensor seq_lens, Tensor query_start_loc, Tensor(a!) out, int max_q_len, "
       "float softmax_scale, int num_seqs, Tensor? k_scale=None, Tensor? v_scale=None, "
       "Tensor(b!)? status=None, Tensor(c!)? workspace=None) -> ()");
+  m.def(
+      "kv_append_int4(Tensor key, Tensor value, Tensor(a!) k_cache, Tensor(b!) v_cache, "
+      "Tensor slot_mapping, Tensor(c!)? status=None) -> ()");
+  m.def(
+      "kv_load_int4(Tensor k_cache, Tensor v_cache, Tensor slot_mapping, Tensor(a!) key, "
+      "Tensor(b!) value, Tensor(c!)? status=None) -> ()");
+  m.def(
+      "paged_decode_int4(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, "
+      "Tensor seq_lens, Tensor(a!) out, int num_parts, int part_tokens, float softmax_scale, "
+      "Tensor(b!)? workspace=None, Tensor(c!)? status=None) -> ()");
+  m.def(
+      "paged_prefill_int4(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, "
+      "Tensor seq_lens, Tensor query_start_loc, Tensor(a!) out, int max_q_len, "
+      "float softmax_scale, int num_seqs, Tensor(b!)? status=None) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(b200, CUDA, m) {
   m.impl("kv_append", &kv_append);
   m.impl("paged_decode", &paged_decode);
   m.impl("paged_prefill", &paged_prefill);
+  m.impl("kv_append_int4", &kv_append_int4);
+  m.impl("kv_load_int4", &kv_load_int4);
+  m.impl("paged_decode_int4", &paged_decode_int4);
+  m.impl("paged_prefill_int4", &paged_prefill_int4);
 }
 
 TORCH_LIBRARY_IMPL(b200, Meta, m) {
   m.impl("kv_append", &kv_append_meta);
   m.impl("paged_decode", &paged_decode_meta);
   m.impl("paged_prefill", &paged_prefill_meta);
+  m.impl("kv_append_int4", &kv_append_int4_meta);
+  m.impl("kv_load_int4", &kv_load_int4_meta);
+  m.impl("paged_decode_int4", &paged_decode_int4_meta);
+  m.impl("paged_prefill_int4", &paged_prefill_int4_meta);
 }
