@@ -697,6 +697,72 @@ int validate_int4_cache(const b200_int4_cache* c, b200::Int4Cache* out) {
   return B200_OK;
 }
 
+// Tensor map over one 4-bit cache tensor's codes (scales = false) or scales, for
+// boxes of `rows` slots (see b200::Int4Maps). `key.dtype` keeps its keys apart
+// from the other maps'.
+int int4_tensor_map(const uint8_t* base, const b200::Int4Cache& c, bool scales, int rows,
+                    CUtensorMap* out) {
+  MapKey key;
+  std::memset(&key, 0, sizeof(key));
+  key.ptr = reinterpret_cast<uint64_t>(base);
+  key.dims[0] = c.num_kv_heads;
+  key.dims[1] = c.block_size;
+  key.dims[2] = c.num_blocks;
+  key.dims[3] = rows;
+  key.strides[0] = c.block_stride;
+  key.dtype = scales ? 2001 : 2000;
+  {
+    std::lock_guard<std::mutex> lock(g_map_mu);
+    auto it = map_cache().find(key);
+    if (it != map_cache().end()) {
+      *out = it->second;
+      return B200_OK;
+    }
+  }
+  auto fn = encode_fn();
+  if (fn == nullptr)
+    return fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+  const cuuint64_t heads = c.num_kv_heads, bs = c.block_size, blocks = c.num_blocks;
+  const cuuint64_t stride = c.block_stride;
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  CUtensorMap m;
+  CUresult r;
+  if (scales) {
+    const cuuint64_t dims[3] = {bs * b200::kInt4ScaleBytes, heads, blocks};
+    const cuuint64_t strides[2] = {bs * b200::kInt4ScaleBytes, stride};
+    const cuuint32_t box[3] = {(cuuint32_t)(rows * b200::kInt4ScaleBytes), 1, 1};
+    r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3,
+           const_cast<uint8_t*>(base) + heads * bs * b200::kInt4CodeBytes, dims, strides, box, one,
+           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  } else {
+    const cuuint64_t dims[4] = {b200::kInt4CodeBytes, bs, heads, blocks};
+    const cuuint64_t strides[3] = {b200::kInt4CodeBytes, bs * b200::kInt4CodeBytes, stride};
+    const cuuint32_t box[4] = {b200::kInt4CodeBytes, (cuuint32_t)rows, 1, 1};
+    r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, box,
+           one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  }
+  if (r != CUDA_SUCCESS)
+    return fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled (int4) failed with CUresult " +
+                                   std::to_string(static_cast<int>(r)));
+  {
+    std::lock_guard<std::mutex> lock(g_map_mu);
+    if (map_cache().size() > 4096) map_cache().clear();
+    map_cache().emplace(key, m);
+  }
+  *out = m;
+  return B200_OK;
+}
+
+int int4_maps(const b200::Int4Cache& c, int rows, b200::Int4Maps* maps) {
+  int rc;
+  if ((rc = int4_tensor_map(c.k, c, false, rows, &maps->kc)) != B200_OK) return rc;
+  if ((rc = int4_tensor_map(c.k, c, true, rows, &maps->ks)) != B200_OK) return rc;
+  if ((rc = int4_tensor_map(c.v, c, false, rows, &maps->vc)) != B200_OK) return rc;
+  return int4_tensor_map(c.v, c, true, rows, &maps->vs);
+}
+
 int validate_int4_dtype(int32_t dtype) {
   if (dtype != B200_DTYPE_BFLOAT16 && dtype != B200_DTYPE_FLOAT16)
     return fail(B200_ERR_UNSUPPORTED, "dtype must be float16 or bfloat16");
@@ -807,25 +873,37 @@ int b200_paged_decode_int4(const void* q, int64_t q_seq_stride, int64_t q_head_s
                 "decode workspace too small: need " + std::to_string(need) + " bytes");
   if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 255))
     return fail(B200_ERR_INVALID_ARGUMENT, "decode workspace must be 256-byte aligned");
-  b200::Int4AttnParams p{};
+  b200::Int4DecodeParams p{};
   p.q = q;
-  p.q_token_stride = q_seq_stride;
+  p.q_seq_stride = q_seq_stride;
   p.q_head_stride = q_head_stride;
   p.block_tables = block_tables;
   p.block_table_stride = block_table_stride;
   p.max_blocks = max_blocks;
   p.seq_lens = seq_lens;
-  p.plan_tokens = (int64_t)plan->num_parts * plan->part_tokens;
   p.out = out;
-  p.out_token_stride = out_seq_stride;
+  p.out_seq_stride = out_seq_stride;
   p.out_head_stride = out_head_stride;
-  p.num_seqs = num_seqs;
-  p.num_q_tokens = num_seqs;
-  p.num_q_heads = num_q_heads;
+  const int64_t slots = (int64_t)num_seqs * num_q_heads * plan->num_parts;
+  p.part_o = need > 0 ? static_cast<float*>(workspace) : nullptr;
+  p.part_lse = need > 0 ? reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                                   (slots * b200::kHeadDim * 4 + 255) / 256 * 256)
+                        : nullptr;
+  p.num_parts = plan->num_parts;
+  p.part_tokens = plan->part_tokens;
+  p.block_size = c.block_size;
+  p.box_rows = c.block_size % 32 == 0 && plan->part_tokens % 32 == 0 ? 32 : 16;
   p.group = group;
+  p.num_seqs = num_seqs;
+  p.num_q_heads = num_q_heads;
+  p.num_kv_heads = c.num_kv_heads;
+  p.num_blocks = c.num_blocks;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.status = status;
-  cudaError_t e = b200::launch_int4_attention(c, p, dtype, static_cast<cudaStream_t>(stream));
+  b200::Int4Maps maps;
+  if ((rc = int4_maps(c, p.box_rows, &maps)) != B200_OK) return rc;
+  cudaError_t e =
+      b200::launch_paged_decode_int4(maps, p, dtype, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "int4 paged decode launch");
   return B200_OK;
 }

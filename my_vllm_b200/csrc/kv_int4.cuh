@@ -70,6 +70,42 @@ struct Int4AttnParams {
   int32_t* status;
 };
 
+// Tensor maps of a cache pair (built by the C ABI layer). Codes: (byte of a row
+// 64, slot, head, page), box 64 x box_rows x 1 x 1, 64-byte swizzle. Scales:
+// (byte of a head's scales 8 block_size, head, page), box 8 box_rows x 1 x 1.
+struct Int4Maps {
+  CUtensorMap kc, ks, vc, vs;
+};
+
+struct Int4DecodeParams {
+  const void* q;
+  int64_t q_seq_stride;
+  int64_t q_head_stride;
+  const int32_t* block_tables;
+  int64_t block_table_stride;
+  int max_blocks;
+  const int32_t* seq_lens;
+  void* out;
+  int64_t out_seq_stride;
+  int64_t out_head_stride;
+  float* part_o;    // [num_seqs, num_q_heads, num_parts, head_dim]
+  float* part_lse;  // [num_seqs, num_q_heads, num_parts], log2 domain
+  int num_parts;
+  int part_tokens;
+  int block_size;
+  int box_rows;  // slots a TMA box takes: 32 where pages and partitions are multiples of it, or 16
+  int group;
+  int num_seqs;
+  int num_q_heads;
+  int num_kv_heads;
+  int64_t num_blocks;
+  float scale_log2;
+  int32_t* status;
+};
+
+cudaError_t launch_paged_decode_int4(const Int4Maps& maps, const Int4DecodeParams& p, int dtype,
+                                     cudaStream_t stream);
+
 cudaError_t launch_int4_attention(const Int4Cache& cache, const Int4AttnParams& p, int dtype,
                                   cudaStream_t stream);
 
