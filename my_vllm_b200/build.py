@@ -27,7 +27,6 @@ TORCH_OPS_SOURCES = ("torch_ops.cpp",)
 SOURCES = (
     "kv_append.cu",
     "kv_int4.cu",
-    "paged_int4.cu",
     "paged_decode_int4.cu",
     "rope_append.cu",
     "paged_decode.cu",

@@ -937,7 +937,8 @@ int b200_paged_prefill_int4(const void* q, int64_t q_token_stride, int64_t q_hea
       (q_token_stride | q_head_stride | out_token_stride | out_head_stride) & 7)
     return fail(B200_ERR_INVALID_ARGUMENT,
                 "q/out must be 16-byte aligned with strides that are multiples of 8");
-  b200::Int4AttnParams p{};
+  if (max_blocks == 0) return fail(B200_ERR_INVALID_ARGUMENT, "block_tables has no columns");
+  b200::PrefillParams p{};
   p.q = q;
   p.q_token_stride = q_token_stride;
   p.q_head_stride = q_head_stride;
@@ -949,13 +950,31 @@ int b200_paged_prefill_int4(const void* q, int64_t q_token_stride, int64_t q_hea
   p.out = out;
   p.out_token_stride = out_token_stride;
   p.out_head_stride = out_head_stride;
-  p.num_seqs = num_seqs;
-  p.num_q_tokens = num_q_tokens;
-  p.num_q_heads = num_q_heads;
+  p.block_size = c.block_size;
   p.group = group;
+  p.num_q_heads = num_q_heads;
+  p.num_blocks = c.num_blocks;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.status = status;
-  cudaError_t e = b200::launch_int4_attention(c, p, dtype, static_cast<cudaStream_t>(stream));
+  b200::Int4Maps maps;
+  if ((rc = int4_maps(c, b200::kTileTokens, &maps)) != B200_OK) return rc;
+  // Q and whole output tiles by TMA under the conditions of b200_paged_prefill
+  CUtensorMap mq, mo;
+  std::memset(&mq, 0, sizeof(mq));
+  std::memset(&mo, 0, sizeof(mo));
+  p.q_tma = p.o_tma = 128 % group == 0 ? 1 : 0;
+  if (p.q_tma && q_tensor_map(q, dtype, num_q_heads, num_q_tokens, q_head_stride, q_token_stride,
+                              group, &mq) != B200_OK) {
+    p.q_tma = 0;
+    g_last_error.clear();
+  }
+  if (p.o_tma && q_tensor_map(out, dtype, num_q_heads, num_q_tokens, out_head_stride,
+                              out_token_stride, group, &mo) != B200_OK) {
+    p.o_tma = 0;
+    g_last_error.clear();
+  }
+  cudaError_t e = b200::launch_paged_prefill_int4(maps, mq, mo, p, dtype, c.num_kv_heads, num_seqs,
+                                                  max_q_len, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "int4 paged prefill launch");
   return B200_OK;
 }

@@ -47,29 +47,6 @@ cudaError_t launch_load_kvcache_int4(const Int4Cache& cache, const void* slots, 
                                      void* value, int64_t value_row_stride, int dtype,
                                      int32_t* status, cudaStream_t stream);
 
-// Attention over a 4-bit cache. Decode: one query row per sequence
-// (query_start_loc NULL); prefill: rows [query_start_loc[s], query_start_loc[s+1]).
-struct Int4AttnParams {
-  const void* q;
-  int64_t q_token_stride;
-  int64_t q_head_stride;
-  const int32_t* block_tables;
-  int64_t block_table_stride;
-  int max_blocks;  // valid columns of a block-table row
-  const int32_t* seq_lens;
-  const int32_t* query_start_loc;
-  int64_t plan_tokens;  // decode: what the plan covers of each sequence
-  void* out;
-  int64_t out_token_stride;
-  int64_t out_head_stride;
-  int num_seqs;
-  int num_q_tokens;
-  int num_q_heads;
-  int group;  // q heads per KV head
-  float scale_log2;  // softmax_scale * log2(e)
-  int32_t* status;
-};
-
 // Tensor maps of a cache pair (built by the C ABI layer). Codes: (byte of a row
 // 64, slot, head, page), box 64 x box_rows x 1 x 1, 64-byte swizzle. Scales:
 // (byte of a head's scales 8 block_size, head, page), box 8 box_rows x 1 x 1.
@@ -105,8 +82,5 @@ struct Int4DecodeParams {
 
 cudaError_t launch_paged_decode_int4(const Int4Maps& maps, const Int4DecodeParams& p, int dtype,
                                      cudaStream_t stream);
-
-cudaError_t launch_int4_attention(const Int4Cache& cache, const Int4AttnParams& p, int dtype,
-                                  cudaStream_t stream);
 
 }  // namespace b200

@@ -135,9 +135,9 @@ def attention(q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, scal
             sc = np.where(visible, sc, -np.inf)
             km = np.where(visible, (np.abs(x) @ np.abs(k[:, h // group]).T) * scale, 0.0)
             tm = np.where(visible, (np.abs(x) @ wide[:, h // group].T) * scale, 0.0)
-            p = np.exp(sc - sc.max(axis=1, keepdims=True))
-            p /= p.sum(axis=1, keepdims=True)
-            p = np.where(visible, p, 0.0)
+            top = sc.max(axis=1, keepdims=True)
+            p = np.exp(sc - np.where(np.isneginf(top), 0.0, top))
+            p /= np.maximum(p.sum(axis=1, keepdims=True), 1e-300)  # no token: a row of zeros
             vv = v[:, h // group]
             out[q0:q1, h] = p @ vv
             mass[q0:q1, h] = p @ (np.abs(vv) + v_step[:, h // group])

@@ -361,6 +361,40 @@ def test_prefill_bad_pages_are_reported(cuda_device):
     assert_within(out[20:], ref[20:], tol[20:])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_prefill_nan_reaches_the_rows_that_see_it(cuda_device, dtype):
+    c = Case([90, 20], [150, 20], 8, 2, 16, dtype, seed=2)
+    ref, bounds = c.reference()
+    token = 100  # of sequence 0: rows 40 and up see it
+    for cache, group in ((c.v, 1), (c.k, 3)):
+        pages = int4.Pages(cache.numpy())
+        page, row = divmod(c.slots[0][token], 16)
+        held = pages.scales[page, 1, row].copy()
+        pages.scales[page, 1, row].view(np.uint16)[group] = 0x7FC0
+        out = _prefill(c, cuda_device).cpu().double()
+        bad = torch.zeros(out.shape, dtype=torch.bool)
+        if cache is c.v:  # its group of columns; the other columns as if nothing were there
+            bad[40:90, 4:, 32:64] = True
+            clean = bad
+        else:
+            bad[40:90, 4:] = True
+        assert torch.equal(out.isnan(), bad)
+        good = out.masked_fill(bad, 0.0)
+        want = np.where(bad.numpy(), 0.0, ref)
+        assert_within(good, want, prefill_tolerance(ref, bounds, dtype))
+        pages.scales[page, 1, row] = held
+    assert clean.any()
+
+
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (5, 1)])
+def test_prefill_rows_that_see_nothing(cuda_device, hq, hkv):
+    # more query rows than keys: the first rows stand before every key
+    c = Case([150, 40, 3], [100, 40, 16], hq, hkv, 16, torch.bfloat16, seed=12)
+    c.lens[2] = c.kv_lens[2] = 0
+    out = _check_prefill(c, cuda_device)
+    assert (out[:50] == 0).all() and (out[50] != 0).any() and (out[190:] == 0).all()
+
+
 # ----------------------------------------------------------- used together --
 @pytest.mark.parametrize("dtype", TYPES)
 def test_a_prompt_then_steps_of_decoding(cuda_device, dtype):
