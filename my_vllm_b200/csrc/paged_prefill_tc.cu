@@ -693,7 +693,7 @@ __global__ void __launch_bounds__(tc_threads<kKv>(), 1)
     // Warp 10 converts rows 0-63 of every staged tile, warp 11 rows 64-127:
     // chunk c of a row (E4M3 d = 16c .. 16c + 15) -> fp16 chunks 2c', 2c'+1
     // of half c / 4 (c' = c % 4), all 128-byte swizzled like the TMA tiles.
-    const int row0 = (warp - kTcConvWarp0) * (kTcKv / kConvWarps);
+    const int row0 = (warp - kTcConvWarp0) * (kTcKv / 2);
     const int c = lane & 7;
     const int h = c >> 2;
     const int c2 = (c & 3) * 2;
@@ -714,7 +714,7 @@ __global__ void __launch_bounds__(tc_threads<kKv>(), 1)
       const uint8_t* raw = smem + L::kRaw0 + (i & 1) * kTcRawTileBytes;
       uint8_t* dst = smem + (is_v ? kTcV0 : kTcK0) + st * kTcTileBytes + h * kTcHalf;
 #pragma unroll 4
-      for (int it = 0; it < kTcKv / kConvWarps / 4; ++it) {
+      for (int it = 0; it < kTcKv / 2 / 4; ++it) {
         const int r = row0 + it * 4 + (lane >> 3);
         const uint4 w = *reinterpret_cast<const uint4*>(raw + swz128(r, c));
         uint4 lo, hi;

@@ -249,20 +249,50 @@ void paged_prefill(const at::Tensor& q, const at::Tensor& k_cache, const at::Ten
 }
 
 // ------------------------------------------------------------ 4-bit caches --
+// These operators are called without checks of their own in Python: theirs
+// raise ValueError and TypeError, in the CUDA and in the Meta (FakeTensor)
+// kernels alike, and the CPU kernels refuse.
+void check_int4(int rc, const char* what) {
+  TORCH_CHECK_VALUE(rc != B200_ERR_INVALID_ARGUMENT, what, ": ", b200_last_error());
+  TORCH_CHECK(rc == B200_OK, what, ": ", b200_last_error());
+}
+
+using Tensors = std::initializer_list<std::reference_wrapper<const at::Tensor>>;
+using Options = std::initializer_list<std::reference_wrapper<const std::optional<at::Tensor>>>;
+
+// (a FakeTensor is a meta tensor to the Meta kernels)
+void require_one_device(const at::Tensor& first, Tensors rest, Options opt) {
+  TORCH_CHECK_VALUE(first.device().is_cuda() || first.device().is_meta(),
+                    "tensors must be CUDA tensors (the B200 path has no CPU fallback)");
+  for (const at::Tensor& t : rest)
+    TORCH_CHECK_VALUE(t.device() == first.device(),
+                      "every tensor must be a CUDA tensor on one device");
+  for (const std::optional<at::Tensor>& t : opt)
+    TORCH_CHECK_VALUE(!t.has_value() || t->device() == first.device(),
+                      "every tensor must be a CUDA tensor on one device");
+}
+
+void require_status(const std::optional<at::Tensor>& s) {
+  TORCH_CHECK_TYPE(!s.has_value() || (s->scalar_type() == at::kInt && s->numel() >= 1),
+                   "status must be an int32 tensor");
+}
+
 // The cache pair uint8 [num_blocks, block_size, num_kv_heads, 72]; pages may be
 // strided, the inside of a page is packed.
+void require_int4_caches(const at::Tensor& k, const at::Tensor& v) {
+  TORCH_CHECK_TYPE(k.scalar_type() == at::kByte && v.scalar_type() == at::kByte,
+                   "4-bit caches must both be torch.uint8");
+  TORCH_CHECK_VALUE(k.dim() == 4 && k.sizes() == v.sizes() && k.size(3) == B200_INT4_ROW_BYTES,
+                    "4-bit caches must have shape [num_blocks, block_size, num_kv_heads, 72]");
+  TORCH_CHECK_VALUE(k.strides() == v.strides(),
+                    "key and value caches must have identical strides");
+  TORCH_CHECK_VALUE(k.stride(3) == 1 && k.stride(2) == B200_INT4_ROW_BYTES &&
+                        k.stride(1) == k.size(2) * B200_INT4_ROW_BYTES,
+                    "the pages of a 4-bit cache must be packed");
+  TORCH_CHECK_VALUE(k.size(1) <= INT32_MAX && k.size(2) <= INT32_MAX, "cache too large");
+}
+
 b200_int4_cache int4_cache_desc(const at::Tensor& k, const at::Tensor& v) {
-  require_cuda(k, "k_cache");
-  require_cuda(v, "v_cache");
-  TORCH_CHECK(k.scalar_type() == at::kByte && v.scalar_type() == at::kByte,
-              "b200: 4-bit caches must be uint8");
-  TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes() && k.size(3) == B200_INT4_ROW_BYTES,
-              "b200: 4-bit caches must have shape [pages, block_size, num_kv_heads, 72]");
-  TORCH_CHECK(k.strides() == v.strides(), "b200: key and value caches must have identical strides");
-  TORCH_CHECK(k.stride(3) == 1 && k.stride(2) == B200_INT4_ROW_BYTES &&
-                  k.stride(1) == k.size(2) * B200_INT4_ROW_BYTES,
-              "b200: the pages of a 4-bit cache must be packed");
-  TORCH_CHECK(k.size(1) <= INT32_MAX && k.size(2) <= INT32_MAX, "b200: cache too large");
   b200_int4_cache c{};
   c.k_cache = k.data_ptr();
   c.v_cache = v.data_ptr();
@@ -274,31 +304,31 @@ b200_int4_cache int4_cache_desc(const at::Tensor& k, const at::Tensor& v) {
   return c;
 }
 
-void same_device(const at::Tensor& first,
-                 std::initializer_list<std::reference_wrapper<const at::Tensor>> rest,
-                 std::initializer_list<std::reference_wrapper<const std::optional<at::Tensor>>> opt) {
-  for (const at::Tensor& t : rest)
-    TORCH_CHECK(t.device() == first.device(), "b200: every tensor must be on one device");
-  for (const std::optional<at::Tensor>& t : opt)
-    TORCH_CHECK(!t.has_value() || t->device() == first.device(),
-                "b200: every tensor must be on one device");
+void require_16bit(const at::Tensor& t, const char* what) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, what,
+                   " must be float16/bfloat16");
 }
 
-// The 16-bit rows [tokens, num_kv_heads, 128] of the append and the read-back.
-void require_int4_rows(const at::Tensor& key, const at::Tensor& value, const at::Tensor& cache,
-                       const at::Tensor& slots) {
-  TORCH_CHECK(key.dim() == 3 && key.sizes() == value.sizes() && key.size(1) == cache.size(2) &&
-                  key.size(2) == 128 && key.scalar_type() == value.scalar_type(),
-              "b200: key and value must be [tokens, num_kv_heads, 128] of one type");
-  TORCH_CHECK(key.stride(2) == 1 && value.stride(2) == 1 &&
-                  (key.size(1) == 1 || (key.stride(1) == 128 && value.stride(1) == 128)),
-              "b200: key/value heads must be packed (stride(1) == head_dim)");
-  require_cuda(slots, "slot_mapping");
-  TORCH_CHECK(slots.scalar_type() == at::kInt || slots.scalar_type() == at::kLong,
-              "b200: slot_mapping must be int32 or int64");
-  TORCH_CHECK(slots.dim() == 1 && slots.numel() == key.size(0) &&
-                  (slots.numel() <= 1 || slots.stride(0) == 1),
-              "b200: slot_mapping must be a contiguous 1-D tensor of one slot per token");
+void require_int4_rows(const at::Tensor& key, const at::Tensor& value, const at::Tensor& k_cache,
+                       const at::Tensor& v_cache, const at::Tensor& slots,
+                       const std::optional<at::Tensor>& status) {
+  require_one_device(key, {value, k_cache, v_cache, slots}, {status});
+  require_16bit(key, "key and value");
+  TORCH_CHECK_TYPE(value.scalar_type() == key.scalar_type(),
+                   "key and value must share one float16/bfloat16 dtype");
+  require_int4_caches(k_cache, v_cache);
+  TORCH_CHECK_VALUE(key.dim() == 3 && key.sizes() == value.sizes() &&
+                        key.size(1) == k_cache.size(2) && key.size(2) == 128,
+                    "key and value must be [tokens, num_kv_heads, 128]");
+  TORCH_CHECK_VALUE(key.stride(2) == 1 && value.stride(2) == 1 &&
+                        (key.size(1) == 1 || (key.stride(1) == 128 && value.stride(1) == 128)),
+                    "key/value heads must be packed (stride(1) == head_dim)");
+  TORCH_CHECK_TYPE(slots.scalar_type() == at::kInt || slots.scalar_type() == at::kLong,
+                   "slot_mapping must be int32 or int64");
+  TORCH_CHECK_VALUE(slots.dim() == 1 && slots.numel() == key.size(0) &&
+                        (slots.numel() <= 1 || slots.stride(0) == 1),
+                    "slot_mapping must be a contiguous 1-D tensor of one slot per token");
+  require_status(status);
 }
 
 // Rows of a single token have no stride of their own.
@@ -309,47 +339,72 @@ int64_t row_stride(const at::Tensor& t) {
 void kv_append_int4(const at::Tensor& key, const at::Tensor& value, at::Tensor& k_cache,
                     at::Tensor& v_cache, const at::Tensor& slot_mapping,
                     const std::optional<at::Tensor>& status) {
-  require_cuda(key, "key");
-  require_cuda(value, "value");
+  require_int4_rows(key, value, k_cache, v_cache, slot_mapping, status);
   const b200_int4_cache cache = int4_cache_desc(k_cache, v_cache);
-  require_int4_rows(key, value, k_cache, slot_mapping);
-  same_device(key, {value, k_cache, v_cache, slot_mapping}, {status});
   const c10::cuda::CUDAGuard guard(key.device());
-  check_abi(b200_store_kvcache_int4(key.data_ptr(), row_stride(key), value.data_ptr(),
-                                    row_stride(value), activation_dtype(key.scalar_type()), &cache,
-                                    slot_mapping.data_ptr(),
-                                    slot_mapping.scalar_type() == at::kLong ? 1 : 0, key.size(0),
-                                    status_ptr(status), current_stream(key)),
-            "b200_store_kvcache_int4");
+  check_int4(b200_store_kvcache_int4(key.data_ptr(), row_stride(key), value.data_ptr(),
+                                     row_stride(value), activation_dtype(key.scalar_type()),
+                                     &cache, slot_mapping.data_ptr(),
+                                     slot_mapping.scalar_type() == at::kLong ? 1 : 0, key.size(0),
+                                     status_ptr(status), current_stream(key)),
+             "store_kvcache_int4");
 }
 
 void kv_load_int4(const at::Tensor& k_cache, const at::Tensor& v_cache,
                   const at::Tensor& slot_mapping, at::Tensor& key, at::Tensor& value,
                   const std::optional<at::Tensor>& status) {
-  require_cuda(key, "key");
-  require_cuda(value, "value");
+  require_int4_rows(key, value, k_cache, v_cache, slot_mapping, status);
   const b200_int4_cache cache = int4_cache_desc(k_cache, v_cache);
-  require_int4_rows(key, value, k_cache, slot_mapping);
-  same_device(key, {value, k_cache, v_cache, slot_mapping}, {status});
   const c10::cuda::CUDAGuard guard(key.device());
-  check_abi(b200_load_kvcache_int4(&cache, slot_mapping.data_ptr(),
-                                   slot_mapping.scalar_type() == at::kLong ? 1 : 0, key.size(0),
-                                   key.data_ptr(), row_stride(key), value.data_ptr(),
-                                   row_stride(value), activation_dtype(key.scalar_type()),
-                                   status_ptr(status), current_stream(key)),
-            "b200_load_kvcache_int4");
+  check_int4(b200_load_kvcache_int4(&cache, slot_mapping.data_ptr(),
+                                    slot_mapping.scalar_type() == at::kLong ? 1 : 0, key.size(0),
+                                    key.data_ptr(), row_stride(key), value.data_ptr(),
+                                    row_stride(value), activation_dtype(key.scalar_type()),
+                                    status_ptr(status), current_stream(key)),
+             "load_kvcache_int4");
 }
 
-void require_attention(const at::Tensor& q, const at::Tensor& out, const at::Tensor& block_tables,
-                       const at::Tensor& seq_lens) {
-  require_cuda(q, "q");
-  require_cuda(out, "out");
-  TORCH_CHECK(q.dim() == 3 && out.sizes() == q.sizes() && q.size(2) == 128 && q.stride(2) == 1 &&
-                  out.stride(2) == 1,
-              "b200: q and out must be [tokens, num_q_heads, 128], head_dim contiguous");
-  TORCH_CHECK(out.scalar_type() == q.scalar_type(), "b200: out must have the query dtype");
-  require_block_tables(block_tables);
-  require_int32_vector(seq_lens, "seq_lens");
+void require_int4_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                            const at::Tensor& out, const at::Tensor& block_tables,
+                            const at::Tensor& seq_lens, const std::optional<at::Tensor>& status) {
+  require_16bit(q, "the query over a 4-bit cache");
+  require_int4_caches(k, v);
+  TORCH_CHECK_VALUE(out.scalar_type() == q.scalar_type(),
+                    "query and output must share one dtype");
+  TORCH_CHECK_VALUE(q.dim() == 3 && out.sizes() == q.sizes() && q.stride(2) == 1 &&
+                        out.stride(2) == 1,
+                    "q and out must be [tokens, num_q_heads, head_dim], head_dim contiguous");
+  TORCH_CHECK_VALUE(q.size(2) == 128, "head_dim must be 128");
+  TORCH_CHECK_VALUE(q.size(1) > 0 && k.size(2) > 0 && q.size(1) % k.size(2) == 0,
+                    "num_q_heads must be divisible by num_kv_heads");
+  TORCH_CHECK_TYPE(block_tables.scalar_type() == at::kInt && seq_lens.scalar_type() == at::kInt,
+                   "block_tables and seq_lens must be int32");
+  TORCH_CHECK_VALUE(block_tables.dim() == 2 &&
+                        (block_tables.size(1) <= 1 || block_tables.stride(1) == 1) &&
+                        seq_lens.dim() == 1 && (seq_lens.numel() <= 1 || seq_lens.stride(0) == 1),
+                    "block_tables rows and seq_lens must be contiguous");
+  TORCH_CHECK_VALUE(q.size(0) <= INT32_MAX && q.size(1) <= INT32_MAX &&
+                        block_tables.size(1) <= INT32_MAX,
+                    "too many query rows, heads or pages");
+  require_status(status);
+}
+
+void require_int4_decode(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                         const at::Tensor& block_tables, const at::Tensor& seq_lens,
+                         const at::Tensor& out, int64_t num_parts, int64_t part_tokens,
+                         const std::optional<at::Tensor>& workspace,
+                         const std::optional<at::Tensor>& status) {
+  require_one_device(q, {k_cache, v_cache, block_tables, seq_lens, out}, {workspace, status});
+  require_int4_attention(q, k_cache, v_cache, out, block_tables, seq_lens, status);
+  TORCH_CHECK_VALUE(block_tables.size(0) >= q.size(0) && seq_lens.numel() >= q.size(0),
+                    "block_tables / seq_lens must have one row per sequence");
+  TORCH_CHECK_VALUE(num_parts >= 1 && num_parts <= INT32_MAX && part_tokens >= 1 &&
+                        part_tokens <= INT32_MAX,
+                    "malformed decode plan");
+  TORCH_CHECK_VALUE(!workspace.has_value() || workspace->is_contiguous(),
+                    "workspace must be contiguous");
+  TORCH_CHECK_VALUE(num_parts == 1 || q.size(0) == 0 || workspace.has_value(),
+                    "decode workspace smaller than the plan requires");
 }
 
 void paged_decode_int4(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
@@ -357,31 +412,47 @@ void paged_decode_int4(const at::Tensor& q, const at::Tensor& k_cache, const at:
                        int64_t num_parts, int64_t part_tokens, double softmax_scale,
                        const std::optional<at::Tensor>& workspace,
                        const std::optional<at::Tensor>& status) {
-  require_attention(q, out, block_tables, seq_lens);
-  const int64_t b = q.size(0);
-  TORCH_CHECK(block_tables.size(0) >= b && seq_lens.numel() >= b,
-              "b200: block_tables / seq_lens must have one row per sequence");
-  TORCH_CHECK(num_parts <= INT32_MAX && part_tokens <= INT32_MAX, "b200: malformed decode plan");
+  require_int4_decode(q, k_cache, v_cache, block_tables, seq_lens, out, num_parts, part_tokens,
+                      workspace, status);
   const b200_int4_cache cache = int4_cache_desc(k_cache, v_cache);
-  same_device(q, {k_cache, v_cache, block_tables, seq_lens, out}, {workspace, status});
   void* ws = nullptr;
   int64_t ws_bytes = 0;
   if (workspace.has_value()) {
-    TORCH_CHECK(workspace->is_contiguous(), "b200: workspace must be contiguous");
     ws = workspace->data_ptr();
     ws_bytes = workspace->numel() * workspace->element_size();
   }
   b200_decode_plan plan{static_cast<int32_t>(num_parts), static_cast<int32_t>(part_tokens), 0};
   const c10::cuda::CUDAGuard guard(q.device());
-  check_abi(b200_paged_decode_int4(q.data_ptr(), q.stride(0), q.stride(1),
-                                   activation_dtype(q.scalar_type()), &cache,
-                                   block_tables.data_ptr<int32_t>(), block_tables.stride(0),
-                                   static_cast<int32_t>(block_tables.size(1)),
-                                   seq_lens.data_ptr<int32_t>(), static_cast<int32_t>(b),
-                                   static_cast<int32_t>(q.size(1)), out.data_ptr(), out.stride(0),
-                                   out.stride(1), static_cast<float>(softmax_scale), &plan, ws,
-                                   ws_bytes, status_ptr(status), current_stream(q)),
-            "b200_paged_decode_int4");
+  check_int4(b200_paged_decode_int4(q.data_ptr(), q.stride(0), q.stride(1),
+                                    activation_dtype(q.scalar_type()), &cache,
+                                    block_tables.data_ptr<int32_t>(), block_tables.stride(0),
+                                    static_cast<int32_t>(block_tables.size(1)),
+                                    seq_lens.data_ptr<int32_t>(),
+                                    static_cast<int32_t>(q.size(0)),
+                                    static_cast<int32_t>(q.size(1)), out.data_ptr(),
+                                    out.stride(0), out.stride(1),
+                                    static_cast<float>(softmax_scale), &plan, ws, ws_bytes,
+                                    status_ptr(status), current_stream(q)),
+             "paged_decode");
+}
+
+void require_int4_prefill(const at::Tensor& q, const at::Tensor& k_cache,
+                          const at::Tensor& v_cache, const at::Tensor& block_tables,
+                          const at::Tensor& seq_lens, const at::Tensor& query_start_loc,
+                          const at::Tensor& out, int64_t max_q_len, int64_t num_seqs,
+                          const std::optional<at::Tensor>& status) {
+  require_one_device(q, {k_cache, v_cache, block_tables, seq_lens, query_start_loc, out},
+                     {status});
+  require_int4_attention(q, k_cache, v_cache, out, block_tables, seq_lens, status);
+  TORCH_CHECK_TYPE(query_start_loc.scalar_type() == at::kInt, "query_start_loc must be int32");
+  TORCH_CHECK_VALUE(query_start_loc.dim() == 1 &&
+                        (query_start_loc.numel() <= 1 || query_start_loc.stride(0) == 1),
+                    "query_start_loc must be contiguous");
+  TORCH_CHECK_VALUE(num_seqs >= 0 && num_seqs <= INT32_MAX &&
+                        query_start_loc.numel() >= num_seqs + 1 &&
+                        block_tables.size(0) >= num_seqs && seq_lens.numel() >= num_seqs,
+                    "query_start_loc / block_tables / seq_lens too short for num_seqs");
+  TORCH_CHECK_VALUE(max_q_len >= 0 && max_q_len <= INT32_MAX, "max_q_len out of range");
 }
 
 void paged_prefill_int4(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
@@ -389,46 +460,59 @@ void paged_prefill_int4(const at::Tensor& q, const at::Tensor& k_cache, const at
                         const at::Tensor& query_start_loc, at::Tensor& out, int64_t max_q_len,
                         double softmax_scale, int64_t num_seqs,
                         const std::optional<at::Tensor>& status) {
-  require_attention(q, out, block_tables, seq_lens);
-  require_int32_vector(query_start_loc, "query_start_loc");
-  TORCH_CHECK(num_seqs >= 0 && query_start_loc.numel() >= num_seqs + 1 &&
-                  block_tables.size(0) >= num_seqs && seq_lens.numel() >= num_seqs,
-              "b200: query_start_loc / block_tables / seq_lens too short for num_seqs");
-  TORCH_CHECK(max_q_len <= INT32_MAX && q.size(0) <= INT32_MAX, "b200: too many query rows");
+  require_int4_prefill(q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, out,
+                       max_q_len, num_seqs, status);
   const b200_int4_cache cache = int4_cache_desc(k_cache, v_cache);
-  same_device(q, {k_cache, v_cache, block_tables, seq_lens, query_start_loc, out}, {status});
   const c10::cuda::CUDAGuard guard(q.device());
-  check_abi(b200_paged_prefill_int4(q.data_ptr(), q.stride(0), q.stride(1),
-                                    activation_dtype(q.scalar_type()), &cache,
-                                    block_tables.data_ptr<int32_t>(), block_tables.stride(0),
-                                    static_cast<int32_t>(block_tables.size(1)),
-                                    seq_lens.data_ptr<int32_t>(),
-                                    query_start_loc.data_ptr<int32_t>(),
-                                    static_cast<int32_t>(num_seqs),
-                                    static_cast<int32_t>(q.size(0)),
-                                    static_cast<int32_t>(max_q_len),
-                                    static_cast<int32_t>(q.size(1)), out.data_ptr(), out.stride(0),
-                                    out.stride(1), static_cast<float>(softmax_scale),
-                                    status_ptr(status), current_stream(q)),
-            "b200_paged_prefill_int4");
+  check_int4(b200_paged_prefill_int4(q.data_ptr(), q.stride(0), q.stride(1),
+                                     activation_dtype(q.scalar_type()), &cache,
+                                     block_tables.data_ptr<int32_t>(), block_tables.stride(0),
+                                     static_cast<int32_t>(block_tables.size(1)),
+                                     seq_lens.data_ptr<int32_t>(),
+                                     query_start_loc.data_ptr<int32_t>(),
+                                     static_cast<int32_t>(num_seqs),
+                                     static_cast<int32_t>(q.size(0)),
+                                     static_cast<int32_t>(max_q_len),
+                                     static_cast<int32_t>(q.size(1)), out.data_ptr(),
+                                     out.stride(0), out.stride(1),
+                                     static_cast<float>(softmax_scale), status_ptr(status),
+                                     current_stream(q)),
+             "paged_prefill");
+}
+
+// Meta (FakeTensor) and CPU kernels: the checks alone; on the CPU the first refuses.
+void kv_append_int4_meta(const at::Tensor& key, const at::Tensor& value, at::Tensor& k_cache,
+                         at::Tensor& v_cache, const at::Tensor& slot_mapping,
+                         const std::optional<at::Tensor>& status) {
+  require_int4_rows(key, value, k_cache, v_cache, slot_mapping, status);
+}
+
+void kv_load_int4_meta(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                       const at::Tensor& slot_mapping, at::Tensor& key, at::Tensor& value,
+                       const std::optional<at::Tensor>& status) {
+  require_int4_rows(key, value, k_cache, v_cache, slot_mapping, status);
+}
+
+void paged_decode_int4_meta(const at::Tensor& q, const at::Tensor& k_cache,
+                            const at::Tensor& v_cache, const at::Tensor& block_tables,
+                            const at::Tensor& seq_lens, at::Tensor& out, int64_t num_parts,
+                            int64_t part_tokens, double,
+                            const std::optional<at::Tensor>& workspace,
+                            const std::optional<at::Tensor>& status) {
+  require_int4_decode(q, k_cache, v_cache, block_tables, seq_lens, out, num_parts, part_tokens,
+                      workspace, status);
+}
+
+void paged_prefill_int4_meta(const at::Tensor& q, const at::Tensor& k_cache,
+                             const at::Tensor& v_cache, const at::Tensor& block_tables,
+                             const at::Tensor& seq_lens, const at::Tensor& query_start_loc,
+                             at::Tensor& out, int64_t max_q_len, double, int64_t num_seqs,
+                             const std::optional<at::Tensor>& status) {
+  require_int4_prefill(q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, out,
+                       max_q_len, num_seqs, status);
 }
 
 // ------------------------------------------------ Meta (FakeTensor) kernels --
-void kv_append_int4_meta(const at::Tensor&, const at::Tensor&, at::Tensor&, at::Tensor&,
-                         const at::Tensor&, const std::optional<at::Tensor>&) {}
-
-void kv_load_int4_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, at::Tensor&,
-                       at::Tensor&, const std::optional<at::Tensor>&) {}
-
-void paged_decode_int4_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&,
-                            const at::Tensor&, const at::Tensor&, at::Tensor&, int64_t, int64_t,
-                            double, const std::optional<at::Tensor>&,
-                            const std::optional<at::Tensor>&) {}
-
-void paged_prefill_int4_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&,
-                             const at::Tensor&, const at::Tensor&, const at::Tensor&, at::Tensor&,
-                             int64_t, double, int64_t, const std::optional<at::Tensor>&) {}
-
 void kv_append_meta(const at::Tensor&, const at::Tensor&, at::Tensor&, at::Tensor&,
                     const at::Tensor&, const std::optional<at::Tensor>&,
                     const std::optional<at::Tensor>&, const std::optional<at::Tensor>&) {}
@@ -492,6 +576,13 @@ TORCH_LIBRARY_IMPL(b200, Meta, m) {
   m.impl("kv_append", &kv_append_meta);
   m.impl("paged_decode", &paged_decode_meta);
   m.impl("paged_prefill", &paged_prefill_meta);
+  m.impl("kv_append_int4", &kv_append_int4_meta);
+  m.impl("kv_load_int4", &kv_load_int4_meta);
+  m.impl("paged_decode_int4", &paged_decode_int4_meta);
+  m.impl("paged_prefill_int4", &paged_prefill_int4_meta);
+}
+
+TORCH_LIBRARY_IMPL(b200, CPU, m) {
   m.impl("kv_append_int4", &kv_append_int4_meta);
   m.impl("kv_load_int4", &kv_load_int4_meta);
   m.impl("paged_decode_int4", &paged_decode_int4_meta);

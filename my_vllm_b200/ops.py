@@ -179,38 +179,12 @@ def int4_cache_shape(num_blocks: int, block_size: int, num_kv_heads: int,
     return (num_blocks, block_size, num_kv_heads, INT4_ROW_BYTES)
 
 
-def _check_int4_caches(k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
-    if k_cache.dtype != INT4_DTYPE or v_cache.dtype != INT4_DTYPE:
-        raise TypeError("4-bit caches must both be torch.uint8")
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.size(3) != INT4_ROW_BYTES:
-        raise ValueError("4-bit caches must have shape [num_blocks, block_size, num_kv_heads, "
-                         f"{INT4_ROW_BYTES}]")
-    if k_cache.stride() != v_cache.stride():
-        raise ValueError("key and value caches must have identical strides")
-    if k_cache.stride()[1:] != (k_cache.size(2) * INT4_ROW_BYTES, INT4_ROW_BYTES, 1):
-        raise ValueError("the pages of a 4-bit cache must be packed")
-
-
-def _check_int4_rows(key, value, k_cache, v_cache, slot_mapping) -> None:
-    for name, t in (("key", key), ("value", value), ("k_cache", k_cache),
-                    ("v_cache", v_cache), ("slot_mapping", slot_mapping)):
-        _require_cuda(name, t)
-        if t.device != key.device:
-            raise ValueError("every tensor must be on one device")
-    if key.dtype not in _DTYPES or value.dtype != key.dtype:
-        raise TypeError("key and value must share one float16/bfloat16 dtype")
-    _check_int4_caches(k_cache, v_cache)
-    if (key.dim() != 3 or value.shape != key.shape or key.size(1) != k_cache.size(2)
-            or key.size(2) != INT4_HEAD_DIM):
-        raise ValueError("key and value must be [tokens, num_kv_heads, 128]")
-    for name, t in (("key", key), ("value", value)):
-        if t.stride(2) != 1 or (t.size(1) > 1 and t.stride(1) != INT4_HEAD_DIM):
-            raise ValueError(f"{name} heads must be packed (stride(1) == head_dim)")
-    if slot_mapping.dtype not in (torch.int32, torch.int64):
-        raise TypeError("slot_mapping must be int32 or int64")
-    if (slot_mapping.dim() != 1 or slot_mapping.numel() != key.size(0)
-            or (slot_mapping.numel() > 1 and slot_mapping.stride(0) != 1)):
-        raise ValueError("slot_mapping must be a contiguous 1-D tensor of one slot per token")
+@functools.lru_cache(maxsize=1)
+def _int4_ops():
+    """The 4-bit caches' operators: they check their arguments themselves."""
+    ops = _ops()
+    return (ops.kv_append_int4.default, ops.kv_load_int4.default,
+            ops.paged_decode_int4.default, ops.paged_prefill_int4.default)
 
 
 def store_kvcache_int4(
@@ -230,10 +204,7 @@ def store_kvcache_int4(
     (1 / s))``, reciprocal and product rounded to fp32: they stand for
     ``s * (code - 8)``. The 4-bit counterpart of ``store_kvcache``; a slot must
     not be named twice in one call (its row would be a mixture of both)."""
-    _check_int4_rows(key, value, k_cache, v_cache, slot_mapping)
-    if key.size(0) == 0:
-        return
-    _ops().kv_append_int4(key, value, k_cache, v_cache, slot_mapping, status)
+    _int4_ops()[0](key, value, k_cache, v_cache, slot_mapping, status)
 
 
 def load_kvcache_int4(
@@ -248,10 +219,7 @@ def load_kvcache_int4(
     """Read 4-bit cache slots back into the rows of ``key`` and ``value``
     (``[tokens, num_kv_heads, 128]``, float16 or bfloat16, in place), the way
     back of ``store_kvcache_int4``: rows of slot -1 stay as they are."""
-    _check_int4_rows(key, value, k_cache, v_cache, slot_mapping)
-    if key.size(0) == 0:
-        return
-    _ops().kv_load_int4(k_cache, v_cache, slot_mapping, key, value, status)
+    _int4_ops()[1](k_cache, v_cache, slot_mapping, key, value, status)
 
 
 def qk_norm_rope_append(
@@ -595,13 +563,18 @@ def paged_decode(
     """Decode attention for ``q [B, Hq, D]`` into ``out [B, Hq, D]`` (in place).
     With FP8 caches ``k_scale`` / ``v_scale`` dequantise K and V; 4-bit caches
     (``torch.uint8``, planned with ``kv_int4``) carry their own scales."""
+    if k_cache.dtype == INT4_DTYPE and q.dtype != INT4_DTYPE:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError("k_scale / v_scale apply to FP8 caches only")
+        _int4_ops()[2](q, k_cache, v_cache, block_tables, seq_lens, out, plan.num_parts,
+                       plan.part_tokens, softmax_scale, workspace, status)
+        return out
     for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache),
                     ("block_tables", block_tables), ("seq_lens", seq_lens), ("out", out)):
         _require_cuda(name, t)
     if q.dim() != 3 or out.shape != q.shape or q.stride(2) != 1 or out.stride(2) != 1:
         raise ValueError("q and out must be [tokens, num_q_heads, head_dim], head_dim contiguous")
-    int4 = k_cache.dtype == INT4_DTYPE
-    if (q.dtype != k_cache.dtype and k_cache.dtype != FP8_DTYPE and not int4) or out.dtype != q.dtype:
+    if (q.dtype != k_cache.dtype and k_cache.dtype != FP8_DTYPE) or out.dtype != q.dtype:
         raise ValueError("query, output and caches must share one dtype")
     if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32:
         raise TypeError("block_tables and seq_lens must be int32")
@@ -610,35 +583,16 @@ def paged_decode(
     B = q.size(0)
     if block_tables.size(0) < B or seq_lens.numel() < B:
         raise ValueError("block_tables / seq_lens must have one row per sequence")
-    if int4:
-        _check_int4_attention(q, k_cache, v_cache, k_scale, v_scale)
-    else:
-        paged_cache_desc(k_cache, v_cache, q.dtype, k_scale, v_scale)  # cached layout checks
+    paged_cache_desc(k_cache, v_cache, q.dtype, k_scale, v_scale)  # cached layout checks
     if plan.workspace_bytes:
         if workspace is None or workspace.numel() * workspace.element_size() < plan.workspace_bytes:
             raise ValueError("decode workspace smaller than the plan requires")
     else:
         workspace = None
-    if int4:
-        _ops().paged_decode_int4(q, k_cache, v_cache, block_tables, seq_lens, out, plan.num_parts,
-                                 plan.part_tokens, float(softmax_scale), workspace, status)
-        return out
     _ops().paged_decode(q, k_cache, v_cache, block_tables, seq_lens, out, plan.num_parts,
                         plan.part_tokens, float(softmax_scale), workspace, k_scale, v_scale,
                         status)
     return out
-
-
-def _check_int4_attention(q, k_cache, v_cache, k_scale, v_scale) -> None:
-    if q.dtype not in _DTYPES:
-        raise TypeError("a 4-bit cache needs a float16/bfloat16 query")
-    _check_int4_caches(k_cache, v_cache)
-    if k_scale is not None or v_scale is not None:
-        raise ValueError("k_scale / v_scale apply to FP8 caches only")
-    if q.size(2) != INT4_HEAD_DIM:
-        raise ValueError("head_dim must be 128")
-    if q.size(1) == 0 or q.size(1) % k_cache.size(2):
-        raise ValueError("num_q_heads must be divisible by num_kv_heads")
 
 
 def paged_prefill(
@@ -664,14 +618,20 @@ def paged_prefill(
     error) lets units much longer than the batch's average work per SM be
     split over several CTAs; launches sharing a workspace must not overlap.
     Prefill over a 4-bit cache (``torch.uint8``) uses none."""
+    if k_cache.dtype == INT4_DTYPE and q.dtype != INT4_DTYPE:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError("k_scale / v_scale apply to FP8 caches only")
+        _int4_ops()[3](q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, out,
+                       max_q_len, softmax_scale,
+                       seq_lens.numel() if num_seqs is None else num_seqs, status)
+        return out
     for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache),
                     ("block_tables", block_tables), ("seq_lens", seq_lens),
                     ("query_start_loc", query_start_loc), ("out", out)):
         _require_cuda(name, t)
     if q.dim() != 3 or out.shape != q.shape or q.stride(2) != 1 or out.stride(2) != 1:
         raise ValueError("q and out must be [tokens, num_q_heads, head_dim], head_dim contiguous")
-    int4 = k_cache.dtype == INT4_DTYPE
-    if (q.dtype != k_cache.dtype and k_cache.dtype != FP8_DTYPE and not int4) or out.dtype != q.dtype:
+    if (q.dtype != k_cache.dtype and k_cache.dtype != FP8_DTYPE) or out.dtype != q.dtype:
         raise ValueError("query, output and caches must share one dtype")
     for name, t in (("block_tables", block_tables), ("seq_lens", seq_lens),
                     ("query_start_loc", query_start_loc)):
@@ -682,11 +642,6 @@ def paged_prefill(
     S = seq_lens.numel() if num_seqs is None else num_seqs
     if query_start_loc.numel() < S + 1 or block_tables.size(0) < S:
         raise ValueError("query_start_loc / block_tables too short for num_seqs")
-    if int4:
-        _check_int4_attention(q, k_cache, v_cache, k_scale, v_scale)
-        _ops().paged_prefill_int4(q, k_cache, v_cache, block_tables, seq_lens, query_start_loc,
-                                  out, int(max_q_len), float(softmax_scale), S, status)
-        return out
     paged_cache_desc(k_cache, v_cache, q.dtype, k_scale, v_scale)  # cached layout checks
     if workspace is not None and workspace.numel() * workspace.element_size() < prefill_workspace_bytes():
         raise ValueError("prefill workspace smaller than prefill_workspace_bytes()")

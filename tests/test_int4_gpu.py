@@ -81,6 +81,28 @@ def test_append_and_read_back_bit_exact(cuda_device, dtype, hkv, bs, wide):
     assert int(status) == 0
 
 
+@pytest.mark.parametrize("shift,gap", [(8, 0), (0, 8), (16, 16)])
+def test_rows_aligned_to_16_bytes_only(cuda_device, shift, gap):
+    g = torch.Generator().manual_seed(7)
+    row = 2 * 128 + gap
+    flat = torch.randn(20 * row + shift, generator=g).half().to(cuda_device)
+    x = flat[shift:].view(20, row)[:, :256].unflatten(1, (2, 128))
+    k = torch.zeros(ops.int4_cache_shape(2, 16, 2), dtype=torch.uint8, device=cuda_device)
+    v = torch.zeros_like(k)
+    slots = torch.arange(20, device=cuda_device) + 3
+    ops.store_kvcache_int4(x, x, k, v, slots)
+    assert torch.equal(k, v)
+    out = torch.full_like(flat, 9.0)
+    back = out[shift:].view(20, row)[:, :256].unflatten(1, (2, 128))
+    ops.load_kvcache_int4(k, v, slots, back, torch.empty_like(x.contiguous()))
+    want = int4.kv_load_int4(k.cpu().numpy(), slots.cpu().numpy())
+    assert torch.equal(back.cpu(), torch.tensor(want).half())
+    assert (out[shift:].view(20, row)[:, 256:] == 9).all() and (out[:shift] == 9).all()
+    ref = np.zeros(k.shape, np.uint8)
+    int4.kv_append_int4(storage(x), storage(x), ref, ref.copy(), slots.cpu().numpy(), "float16")
+    assert np.array_equal(k.cpu().numpy(), ref)
+
+
 def test_append_dispatches_on_the_cache_type(cuda_device):
     g = torch.Generator().manual_seed(5)
     x = torch.randn(4, 2, 128, generator=g).bfloat16().to(cuda_device)
