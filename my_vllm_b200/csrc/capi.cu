@@ -892,18 +892,14 @@ int b200_paged_decode_int4(const void* q, int64_t q_seq_stride, int64_t q_head_s
   p.num_parts = plan->num_parts;
   p.part_tokens = plan->part_tokens;
   p.block_size = c.block_size;
-  p.box_rows = c.block_size % 32 == 0 && plan->part_tokens % 32 == 0 ? 32 : 16;
   p.group = group;
   p.num_seqs = num_seqs;
   p.num_q_heads = num_q_heads;
   p.num_kv_heads = c.num_kv_heads;
-  p.num_blocks = c.num_blocks;
+  p.cache = c;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.status = status;
-  b200::Int4Maps maps;
-  if ((rc = int4_maps(c, p.box_rows, &maps)) != B200_OK) return rc;
-  cudaError_t e =
-      b200::launch_paged_decode_int4(maps, p, dtype, static_cast<cudaStream_t>(stream));
+  cudaError_t e = b200::launch_paged_decode_int4(p, dtype, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "int4 paged decode launch");
   return B200_OK;
 }

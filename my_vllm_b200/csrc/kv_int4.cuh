@@ -70,17 +70,15 @@ struct Int4DecodeParams {
   int num_parts;
   int part_tokens;
   int block_size;
-  int box_rows;  // slots a TMA box takes: 32 where pages and partitions are multiples of it, or 16
   int group;
   int num_seqs;
   int num_q_heads;
   int num_kv_heads;
-  int64_t num_blocks;
+  Int4Cache cache;
   float scale_log2;
   int32_t* status;
 };
 
-cudaError_t launch_paged_decode_int4(const Int4Maps& maps, const Int4DecodeParams& p, int dtype,
-                                     cudaStream_t stream);
+cudaError_t launch_paged_decode_int4(const Int4DecodeParams& p, int dtype, cudaStream_t stream);
 
 }  // namespace b200

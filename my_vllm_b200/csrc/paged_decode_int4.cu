@@ -11,20 +11,24 @@
 // c 2^-20: one AND per two values makes an operand, no conversion. The odd
 // nibbles' factor of 16 is taken out of q beforehand, and out of O's rows
 // afterwards; the 2^-24 goes into the softmax scale. Products and sums are
-// fp32; -8 sum q is the initial value of the accumulators, and 8 sum w comes
-// from one more MMA per group whose A operand is the constant 8, so both sums
-// see the same rounded weights. Roundings to 16 bits: q (exact: each head is
+// fp32. -8 sum_g ks_g sum q is one bf16 MMA over (group, digit): the scales are
+// bf16 as they are, the four sums of q are split into three bf16 digits. 8 sum
+// w comes from one MMA per group whose A operand is the constant 8, so both
+// sums see the same rounded weights. Roundings to 16 bits: q (exact: each head is
 // scaled to [2^14, 2^15) by a power of two first) and the weights w (fp16,
 // 2^-11). The weights' range is kept in fp16 by a running power of two over
 // the value scales, which takes part in the softmax's running maximum.
 //
 // Work split: one CTA per (sequence, KV head, KV partition), its 4 warps take
-// the partition's 32-token tiles in turn, each with its own ring of stages: 2
-// KiB of K codes, 2 KiB of V codes, 256 bytes of K and of V scales, by TMA (64-
-// byte rows, 64-byte swizzle: ldmatrix without bank conflicts), one mbarrier
-// per stage. The KV tile is the A operand (M = 16 tokens, or 16 values of d),
-// the GQA group's heads are the columns. A K row's 16-byte chunk and a V
-// chunk's 8 columns of 16 bits are both one scale group.
+// the partition's 32-token tiles in turn, each with its own ring of stages (2
+// KiB of K codes, 2 KiB of V codes, 256 bytes of K and of V scales) that it
+// fills itself with 16-byte asynchronous copies: nine instructions a tile, all
+// lanes on consecutive bytes. (TMA boxes, of which a tile of 16-token pages
+// takes eight, cost more issue slots than they saved: 295 us against XX.) Codes
+// land swizzled, 16-byte chunk c of row r at chunk c ^ ((r >> 1) & 3), for
+// ldmatrix without bank conflicts. The KV tile is the A operand (M = 16 tokens,
+// or 16 values of d), the GQA group's heads are the columns. A K row's 16-byte
+// chunk and a V chunk's 8 columns of 16 bits are both one scale group.
 #include <cuda_runtime.h>
 #include <math.h>
 
@@ -41,12 +45,11 @@ constexpr int kStages = 2;
 constexpr int kCodeTile = kTile * kInt4CodeBytes;    // 2 KiB
 constexpr int kScaleTile = kTile * kInt4ScaleBytes;  // 256 B
 constexpr int kVCodes = kCodeTile, kKScales = 2 * kCodeTile, kVScales = kKScales + kScaleTile;
-constexpr int kStageBytes = 2 * (kCodeTile + kScaleTile);  // 4608 = 9 x 512: swizzle-aligned
+constexpr int kStageBytes = 2 * (kCodeTile + kScaleTile);
 constexpr int kRingBytes = kWarps * kStages * kStageBytes;
-constexpr int kMaxSubTiles = kMaxPartTokens / 16;
-constexpr int kSmemBytes = 1024 + kRingBytes + kWarps * kStages * 8 + kMaxSubTiles * 8;
-static_assert(kStageBytes % 512 == 0, "64-byte swizzle pattern repeats every 512 bytes");
-static_assert(kWarps * (32 + 16 * kMergeStride) * 4 + 64 <= kRingBytes, "merge area in the ring");
+constexpr int kMaxSubTiles = kMaxPartTokens / 16 + 1;  // a partition may end in half a tile
+constexpr int kSmemBytes = kRingBytes + kMaxSubTiles * 16;
+static_assert(kWarps * (32 + 16 * kMergeStride) * 4 <= kRingBytes, "merge area in the ring");
 
 // Scores may exceed the running maximum by 2^kSlack before O is rescaled; a
 // weight is then at most 2^(kSlack + kHead) and fp16's normal range still
@@ -56,14 +59,42 @@ constexpr float kHeadroom = 6.f;
 constexpr int kMinScaleExp = 36;  // value scales below 2^-91 are not followed
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                        uint32_t a3, uint32_t b0, uint32_t b1,
-                                        const float (&c)[4]) {
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
-      "{%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same from zero.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1,
+                                              uint32_t a2, uint32_t a3, uint32_t b0,
+                                              uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+      "{%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]),
-        "f"(c[3]));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1,
+                                               uint32_t a2, uint32_t a3, uint32_t b0,
+                                               uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
+      "{%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// 16 bytes from global to shared memory; `bytes` 0 writes zeros and reads nothing.
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
@@ -98,16 +129,11 @@ __device__ __forceinline__ float2 widen<__half>(uint32_t w) {
 // NT: 8-head column tiles (2 for groups of more than 8 q heads).
 template <typename T, int NT>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
-    paged_decode_int4_kernel(const __grid_constant__ CUtensorMap tmap_kc,
-                             const __grid_constant__ CUtensorMap tmap_ks,
-                             const __grid_constant__ CUtensorMap tmap_vc,
-                             const __grid_constant__ CUtensorMap tmap_vs,
-                             const Int4DecodeParams p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kRingBytes);
-  int2* tiles = reinterpret_cast<int2*>(bars + kWarps * kStages);  // (page, row) per box
+    paged_decode_int4_kernel(const Int4DecodeParams p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  // per 16 tokens of the partition: byte offsets of their codes and of their
+  // scales in a cache tensor; codes < 0: no such page, or past the end
+  longlong2* subtiles = reinterpret_cast<longlong2*>(smem + kRingBytes);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -116,34 +142,36 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
   const int part = static_cast<int>(blockIdx.x - unit * parts);
   const int b = static_cast<int>(unit / static_cast<unsigned>(p.num_kv_heads));
   const int kvh = static_cast<int>(unit - (unsigned)b * (unsigned)p.num_kv_heads);
-  const int box = p.box_rows;  // 32, or 16 where pages or partitions end inside a 32-token tile
 
-  if (threadIdx.x == 0) {
-    tma_prefetch_desc(&tmap_kc);
-    tma_prefetch_desc(&tmap_ks);
-    tma_prefetch_desc(&tmap_vc);
-    tma_prefetch_desc(&tmap_vs);
-    for (int i = 0; i < kWarps * kStages; ++i) mbar_init(smem_u32(&bars[i]), 1);
-    mbar_init_fence();
-  }
   // Launched as a programmatic dependent of the append (or whatever ran
   // before): nothing that kernel may have written is read above this line.
   pdl_wait();
 
   const int seq_len = __ldg(p.seq_lens + b);
   const int tok_begin = part * p.part_tokens;
-  // Page and row of every box the partition can have, whatever the length: the
-  // table loads do not wait for it.
+  const int tokens = min(seq_len - tok_begin, p.part_tokens);
   {
     const int32_t* bt = p.block_tables + (int64_t)b * p.block_table_stride;
-    for (int i = threadIdx.x; i < p.part_tokens / box; i += blockDim.x) {
-      const int tok = tok_begin + i * box;
+    for (int i = threadIdx.x; i <= p.part_tokens / 16; i += blockDim.x) {
+      const int tok = tok_begin + i * 16;
       const int col = tok / p.block_size;
+      const int row = kvh * p.block_size + (tok - col * p.block_size);
       const int page = col < p.max_blocks ? __ldg(bt + col) : -1;
-      tiles[i] = make_int2(page, tok - col * p.block_size);
+      longlong2 at = make_longlong2(-1, 0);
+      if (i * 16 < tokens) {
+        if (page >= 0 && page < p.cache.num_blocks) {
+          at.x = page * p.cache.block_stride;
+          at.y = at.x + (int64_t)p.num_kv_heads * p.block_size * kInt4CodeBytes +
+                 row * kInt4ScaleBytes;
+          at.x += row * kInt4CodeBytes;
+        } else {
+          report_status(p.status, B200_STATUS_PAGE_OUT_OF_RANGE);
+        }
+      }
+      subtiles[i] = at;
     }
   }
-  if (tok_begin >= seq_len) {
+  if (tokens <= 0) {
     // partitions past the end are ignored by the reduce; a sequence without
     // tokens gives zeros
     if (part == 0 && p.num_parts == 1) {
@@ -156,15 +184,45 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
   }
   if (part == p.num_parts - 1 && seq_len - tok_begin > p.part_tokens && threadIdx.x == 0)
     report_status(p.status, B200_STATUS_PLAN_EXCEEDED);
-  const int tokens = min(seq_len - tok_begin, p.part_tokens);
   const int ntiles = (tokens + kTile - 1) / kTile;
+  const int my_tiles = ntiles > warp ? (ntiles - warp + kWarps - 1) / kWarps : 0;
 
-  // ---- q: B operands (k = the 8 codes of a K word, n = head), fp16 ----
   const int gr = lane >> 2;
   const int tq = lane & 3;
+  const uint32_t ring = smem_u32(smem) + warp * kStages * kStageBytes;
+  // this lane's place in a copy of 8 rows of codes, and in the copy of the scales
+  const uint32_t copy_to = gr * 64 + ((tq ^ ((gr >> 1) & 3)) << 4);
+  const int64_t lane16 = lane * 16;
+  const uint8_t* scale_from = (lane < 16 ? p.cache.k : p.cache.v) + (lane & 7) * 16;
+
+  auto issue = [&](int j) {
+    const uint32_t dst = ring + (j % kStages) * kStageBytes;
+    const longlong2* at = subtiles + (warp + j * kWarps) * 2;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t from = at[i].x;
+      const uint32_t bytes = from < 0 ? 0 : 16;
+      const int64_t off = (from < 0 ? 0 : from) + lane16;
+      copy16(dst + i * 1024 + copy_to, p.cache.k + off, bytes);
+      copy16(dst + i * 1024 + 512 + copy_to, p.cache.k + off + 512, bytes);
+      copy16(dst + kVCodes + i * 1024 + copy_to, p.cache.v + off, bytes);
+      copy16(dst + kVCodes + i * 1024 + 512 + copy_to, p.cache.v + off + 512, bytes);
+    }
+    const longlong2 mine = at[(lane >> 3) & 1];
+    copy16(dst + kKScales + lane * 16, scale_from + mine.y, mine.x < 0 ? 0 : 16);
+  };
+  __syncthreads();  // the table
+#pragma unroll
+  for (int j = 0; j < kStages - 1; ++j) {
+    if (j < my_tiles) issue(j);
+    copy_commit();
+  }
+
+  // ---- q: B operands (k = the 8 codes of a K word, n = head), fp16 ----
   uint32_t qf[NT][8][2];
-  float qz[NT][4][2];   // -8 2^-24 sum_{d in g} q, per column
+  uint32_t qz[NT][2];   // -8 2^-24 sum_{d in g} q in three bf16 digits, k = 4 digit + g
   float fac[NT][2];     // raw score -> log2 units, per column
+  const float sign = p.scale_log2 < 0.f ? -1.f : 1.f;  // the factor itself stays positive
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int h = nt * 8 + gr;
@@ -187,8 +245,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     // 2^(14 - floor(log2 amax)), and back with the codes' 2^24
     const int e = max(static_cast<int>(__float_as_uint(amax) >> 23), 14);
-    const float up = __uint_as_float(static_cast<uint32_t>(268 - e) << 23);
-    const float down = __uint_as_float(static_cast<uint32_t>(e) << 23) * 1024.f * p.scale_log2;
+    const float up = __uint_as_float(static_cast<uint32_t>(268 - e) << 23) * sign;
+    const float down =
+        __uint_as_float(static_cast<uint32_t>(e) << 23) * 1024.f * fabsf(p.scale_log2);
+    float sums[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       float sum = 0.f;
@@ -204,53 +264,34 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
       qf[nt][2 * g + 1][1] = Elem<__half>::pack(x[g][3] * 0.0625f, x[g][7] * 0.0625f);
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      sum *= -8.f * 5.9604644775390625e-8f;
-      qz[nt][g][0] = __shfl_sync(0xffffffffu, sum, tq * 8);
-      qz[nt][g][1] = __shfl_sync(0xffffffffu, sum, tq * 8 + 4);
+      sums[g] = sum * (-8.f * 5.9604644775390625e-8f);
     }
+    // lane tq: k = 2 tq, 2 tq + 1 are groups (0, 1) for even tq and (2, 3) for odd
+    // tq, digit tq / 2; k + 8 the last digit, in the lanes of digit 0 only
+    float z[2] = {(tq & 1) ? sums[2] : sums[0], (tq & 1) ? sums[3] : sums[1]};
+    float d0[2], d1[2], d2[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      d0[i] = __bfloat162float(__float2bfloat16_rn(z[i]));
+      d1[i] = __bfloat162float(__float2bfloat16_rn(z[i] - d0[i]));
+      d2[i] = z[i] - d0[i] - d1[i];
+    }
+    qz[nt][0] = tq < 2 ? Elem<__nv_bfloat16>::pack(d0[0], d0[1])
+                       : Elem<__nv_bfloat16>::pack(d1[0], d1[1]);
+    qz[nt][1] = tq < 2 ? Elem<__nv_bfloat16>::pack(d2[0], d2[1]) : 0u;
     fac[nt][0] = __shfl_sync(0xffffffffu, down, tq * 8);
     fac[nt][1] = __shfl_sync(0xffffffffu, down, tq * 8 + 4);
   }
 
-  // ---- per-warp TMA ring ----
-  const int my_tiles = ntiles > warp ? (ntiles - warp + kWarps - 1) / kWarps : 0;
-  const uint32_t ring = smem_u32(smem) + warp * kStages * kStageBytes;
-  const uint32_t bar0 = smem_u32(&bars[warp * kStages]);
-  __syncthreads();  // barriers and tile coordinates are visible
-
-  auto issue = [&](int j) {
-    const int t = warp + j * kWarps;
-    const uint32_t dst = ring + (j % kStages) * kStageBytes;
-    const uint32_t bar = bar0 + (j % kStages) * 8;
-    const int boxes = box == kTile || t * kTile + 16 >= tokens ? 1 : 2;
-    mbar_arrive_expect_tx(bar, box * boxes * (2 * kInt4RowBytes));
-    for (int i = 0; i < boxes; ++i) {
-      int2 at = tiles[t * (kTile / box) + i];
-      if (at.x < 0 || at.x >= p.num_blocks) {
-        report_status(p.status, B200_STATUS_PAGE_OUT_OF_RANGE);
-        at.x = -1;  // out of the tensor maps: zeros, never dereferenced
-      }
-      tma_load_4d(dst + i * 1024, &tmap_kc, bar, 0, at.y, kvh, at.x);
-      tma_load_4d(dst + kVCodes + i * 1024, &tmap_vc, bar, 0, at.y, kvh, at.x);
-      tma_load_3d(dst + kKScales + i * 128, &tmap_ks, bar, at.y * kInt4ScaleBytes, kvh, at.x);
-      tma_load_3d(dst + kVScales + i * 128, &tmap_vs, bar, at.y * kInt4ScaleBytes, kvh, at.x);
-    }
-  };
-  int issued = min(my_tiles, kStages);
-  if (lane == 0)
-    for (int j = 0; j < issued; ++j) issue(j);
-
   // ldmatrix row addresses: matrices are (tokens 0-7 | 8-15) x (chunks 2i | 2i + 1)
   const int lrow = (lane & 7) + ((lane >> 3) & 1) * 8;
   const uint32_t loff0 = lrow * 64 + (((lane >> 4) ^ ((lrow >> 1) & 3)) << 4);
-  const uint32_t loff1 = lrow * 64 + (((2 + (lane >> 4)) ^ ((lrow >> 1) & 3)) << 4);
+  const uint32_t loff1 = loff0 ^ 32;
   const float kNegInf = -INFINITY;
-  // constant A operands of 8 sum w: group g's MMA fills rows [4g, 4g + 4) only
-  const uint32_t eight_lo = gr < 4 ? 0x48004800u : 0u;
-  const uint32_t eight_hi = gr < 4 ? 0u : 0x48004800u;
+  constexpr uint32_t kEight = 0x48004800u;
 
   float m_run[NT][2], base[NT][2], l_run[NT][2];
-  float o[NT][8][4], oz[NT][4];
+  float o[NT][8][4], oz[NT][4][4];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     m_run[nt][0] = m_run[nt][1] = kNegInf;
@@ -258,27 +299,23 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
     l_run[nt][0] = l_run[nt][1] = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      oz[nt][i] = 0.f;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) oz[nt][g][i] = 0.f;
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt) o[nt][mt][i] = 0.f;
     }
   }
   uint32_t ref = (kMinScaleExp << 7) | 0x7f;  // bf16 bits: the value scales stay at or below
-  uint32_t poison = 0;                        // groups whose values hold a NaN scale
 
-  int consumed = 0;
-  bool ok = true;
   for (int j = 0; j < my_tiles; ++j) {
-    const bool got = mbar_wait(bar0 + (j % kStages) * 8, (j / kStages) & 1);
-    if (!__all_sync(0xffffffffu, got)) {
-      ok = false;
-      break;
-    }
-    consumed = j + 1;
+    copy_wait<kStages - 2>();
+    __syncwarp();  // tile j has landed for every lane, and every lane is done with j - 1
+    if (j + kStages - 1 < my_tiles) issue(j + kStages - 1);
+    copy_commit();
     const uint32_t kb = ring + (j % kStages) * kStageBytes;
     const int valid = tokens - (warp + j * kWarps) * kTile;
 
-    // ---- scores of 32 tokens: sc[nt][st] = (token g | g + 8) x 2 columns ----
+    // ---- raw scores of 32 tokens: sc[nt][st] = (token g | g + 8) x 2 columns ----
     float sc[NT][2][4];
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
@@ -287,6 +324,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
       ldmatrix_x4(kb + st * 1024 + loff1, kw[4], kw[5], kw[6], kw[7]);
       const uint2 s_lo = lds64(kb + kKScales + (st * 16 + gr) * 8);
       const uint2 s_hi = lds64(kb + kKScales + (st * 16 + gr + 8) * 8);
+      const uint32_t z_lo = (tq & 1) ? s_lo.y : s_lo.x, z_hi = (tq & 1) ? s_hi.y : s_hi.x;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        mma_bf16_first(sc[nt][st], z_lo, z_hi, z_lo, z_hi, qz[nt][0], qz[nt][1]);
       const float ks[4][2] = {{lo_scale(s_lo.x), lo_scale(s_hi.x)},
                               {hi_scale(s_lo.x), hi_scale(s_hi.x)},
                               {lo_scale(s_lo.y), lo_scale(s_hi.y)},
@@ -297,16 +338,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
         const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float zero[4] = {qz[nt][g][0], qz[nt][g][1], qz[nt][g][0], qz[nt][g][1]};
           float acc[4];
-          mma_f16(acc, even_codes(w0), even_codes(w1), odd_codes(w0), odd_codes(w1),
-                  qf[nt][2 * g][0], qf[nt][2 * g][1], zero);
+          mma_f16_first(acc, even_codes(w0), even_codes(w1), odd_codes(w0), odd_codes(w1),
+                        qf[nt][2 * g][0], qf[nt][2 * g][1]);
           mma_f16(acc, even_codes(v0), even_codes(v1), odd_codes(v0), odd_codes(v1),
-                  qf[nt][2 * g + 1][0], qf[nt][2 * g + 1][1], acc);
+                  qf[nt][2 * g + 1][0], qf[nt][2 * g + 1][1]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            sc[nt][st][i] = g == 0 ? ks[g][i >> 1] * acc[i]
-                                   : fmaf(ks[g][i >> 1], acc[i], sc[nt][st][i]);
+          for (int i = 0; i < 4; ++i) sc[nt][st][i] = fmaf(ks[g][i >> 1], acc[i], sc[nt][st][i]);
         }
       }
     }
@@ -317,12 +355,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
     for (int st = 0; st < 2; ++st)
 #pragma unroll
       for (int i = 0; i < 2; ++i) vs[st][i] = lds64(kb + kVScales + (st * 16 + i * 8 + gr) * 8);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int st = 0; st < 2; ++st)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[nt][st][i] *= fac[nt][i & 1];
+    // the four lanes of a token look at one each of its row's four tokens
+    uint2 look = lds64(kb + kVScales + (tq * 8 + gr) * 8);
     if (valid < kTile) {
       // rows past the end may be any bytes; their codes are finite whatever they
       // are, so a weight of exactly 0 needs the scale cleared
@@ -335,13 +369,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) sc[nt][st][2 * i] = sc[nt][st][2 * i + 1] = kNegInf;
           }
+      if (tq * 8 + gr >= valid) look = make_uint2(0, 0);
     }
 
     // ---- running maximum and value exponent; both move rarely ----
-    uint32_t vmax = __vmaxu2(__vmaxu2(vs[0][0].x, vs[0][0].y), __vmaxu2(vs[0][1].x, vs[0][1].y));
-    vmax = __vmaxu2(vmax, __vmaxu2(__vmaxu2(vs[1][0].x, vs[1][0].y),
-                                   __vmaxu2(vs[1][1].x, vs[1][1].y)));
-    vmax = max(vmax & 0xffffu, vmax >> 16);
+    const uint32_t vmax2 = __vmaxu2(look.x, look.y);
+    uint32_t vmax = max(vmax2 & 0xffffu, vmax2 >> 16);
     bool moved = vmax > ref || j == 0;
     float mx[NT][2];
 #pragma unroll
@@ -350,35 +383,25 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
       for (int c = 0; c < 2; ++c) {
         mx[nt][c] = fmaxf(fmaxf(sc[nt][0][c], sc[nt][0][2 + c]),
                           fmaxf(sc[nt][1][c], sc[nt][1][2 + c]));
-        moved |= mx[nt][c] > m_run[nt][c] + kSlack;
+        moved |= fmaf(mx[nt][c], fac[nt][c], -kSlack) > m_run[nt][c];
       }
     if (__any_sync(0xffffffffu, moved)) {
-      if (__any_sync(0xffffffffu, vmax > ref)) {
-        vmax = 0;
+      // a scale that is no number spoils its own group's sums only: it is not followed
+      uint32_t top = 0;
 #pragma unroll
-        for (int st = 0; st < 2; ++st)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              uint32_t& w = g < 2 ? vs[st][i].x : vs[st][i].y;
-              const uint32_t s = (g & 1) ? w >> 16 : w & 0xffffu;
-              if (s >= 0x7f80u) {
-                poison |= 1u << g;
-                w &= (g & 1) ? 0x0000ffffu : 0xffff0000u;
-              } else {
-                vmax = max(vmax, s);
-              }
-            }
-        ref = max(ref, __reduce_max_sync(0xffffffffu, vmax) | 0x7fu);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = i < 2 ? look.x : look.y;
+        const uint32_t s = (i & 1) ? w >> 16 : w & 0xffffu;
+        if (s < 0x7f80u) top = max(top, s);
       }
+      ref = max(ref, __reduce_max_sync(0xffffffffu, top) | 0x7fu);
       const float lift = static_cast<float>(static_cast<int>(ref >> 7) - 126) - kHeadroom;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float alpha[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float m = mx[nt][c];
+          float m = mx[nt][c] * fac[nt][c];
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
@@ -390,7 +413,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          oz[nt][i] *= alpha[i & 1];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) oz[nt][g][i] *= alpha[i & 1];
 #pragma unroll
           for (int mt = 0; mt < 8; ++mt) o[nt][mt][i] *= alpha[i & 1];
         }
@@ -404,7 +428,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
       for (int st = 0; st < 2; ++st)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          sc[nt][st][i] = ex2_approx(sc[nt][st][i] - base[nt][i & 1]);
+          sc[nt][st][i] = ex2_approx(fmaf(sc[nt][st][i], fac[nt][i & 1], -base[nt][i & 1]));
           l_run[nt][i & 1] += sc[nt][st][i];
         }
 #pragma unroll
@@ -426,31 +450,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
           const uint32_t b0 = movmatrix_trans(Elem<__half>::pack(pr[0] * f0, pr[1] * f0));
           const uint32_t b1 = movmatrix_trans(Elem<__half>::pack(pr[2] * f1, pr[3] * f1));
           mma_f16(o[nt][2 * g], even_codes(w0), odd_codes(w0), even_codes(w1), odd_codes(w1), b0,
-                  b1, o[nt][2 * g]);
+                  b1);
           mma_f16(o[nt][2 * g + 1], even_codes(v0), odd_codes(v0), even_codes(v1), odd_codes(v1),
-                  b0, b1, o[nt][2 * g + 1]);
-          const uint32_t e = (g & 1) ? eight_hi : eight_lo;
-          if (g < 2)
-            mma_f16(oz[nt], e, 0u, e, 0u, b0, b1, oz[nt]);
-          else
-            mma_f16(oz[nt], 0u, e, 0u, e, b0, b1, oz[nt]);
+                  b0, b1);
+          mma_f16(oz[nt][g], kEight, kEight, kEight, kEight, b0, b1);
         }
       }
     }
-
-    // ---- refill this stage ----
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (issued < my_tiles) {
-      if (lane == 0) issue(issued);
-      ++issued;
-    }
-  }
-
-  if (!ok) {
-    if (lane == 0) report_status(p.status, B200_STATUS_WAIT_TIMEOUT);
-    for (int j = consumed; j < issued; ++j)  // loads still in flight, each wait bounded again
-      mbar_wait(bar0 + (j % kStages) * 8, (j / kStages) & 1);
   }
 
   // ---- merge the warps ----
@@ -462,13 +468,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
       l_run[nt][c] += __shfl_xor_sync(0xffffffffu, l_run[nt][c], 8);
       l_run[nt][c] += __shfl_xor_sync(0xffffffffu, l_run[nt][c], 16);
     }
-  poison = __reduce_or_sync(0xffffffffu, poison);
   __syncthreads();  // every warp is done with the ring
 
   float* ml = reinterpret_cast<float*>(smem);     // [warp][base 16 | sum 16]
   float* mo = ml + kWarps * 32;                   // [warp][16][kMergeStride]
-  uint32_t* mp = reinterpret_cast<uint32_t*>(mo + kWarps * 16 * kMergeStride);
-  if (lane == 0) mp[warp] = poison;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -476,7 +479,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int head = nt * 8 + tq * 2 + c;
-        const float z = __shfl_sync(0xffffffffu, oz[nt][(g >> 1) * 2 + c], (g & 1) * 16 + tq);
+        const float z = oz[nt][g][c];
         if (head < p.group) {
           const float4 row = make_float4(o[nt][2 * g][c] * 16777216.f - z,
                                          o[nt][2 * g][2 + c] * 1048576.f - z,
@@ -491,7 +494,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
       }
     }
   __syncthreads();
-  const uint32_t bad = mp[0] | mp[1] | mp[2] | mp[3];
 
   for (int idx = threadIdx.x; idx < p.group * (kHeadDim / 4); idx += blockDim.x) {
     const int row = idx >> 5;
@@ -513,7 +515,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3)
       acc.w += x.w * f;
       l += ml[w * 32 + 16 + row] * f;
     }
-    const float inv = (bad >> (d >> 5)) & 1u ? __uint_as_float(0x7fc00000u) : 1.f / l;
+    const float inv = 1.f / l;
     acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     const int head = kvh * p.group + row;
     if (p.num_parts == 1) {
@@ -601,12 +603,12 @@ cudaError_t launch_dependent(void (*kernel)(Args...), unsigned grid, int smem, c
 }
 
 template <typename T, int NT>
-cudaError_t launch_typed(const Int4Maps& maps, const Int4DecodeParams& p, unsigned grid,
+cudaError_t launch_typed(const Int4DecodeParams& p, unsigned grid,
                          cudaStream_t stream) {
   auto kernel = paged_decode_int4_kernel<T, NT>;
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kernel), kSmemBytes);
   if (e != cudaSuccess) return e;
-  e = launch_dependent(kernel, grid, kSmemBytes, stream, maps.kc, maps.ks, maps.vc, maps.vs, p);
+  e = launch_dependent(kernel, grid, kSmemBytes, stream, p);
   if (e != cudaSuccess || p.num_parts == 1) return e;
   return launch_dependent(int4_reduce_kernel<T>, (unsigned)p.num_seqs * (unsigned)p.num_q_heads, 0,
                           stream, p);
@@ -614,17 +616,16 @@ cudaError_t launch_typed(const Int4Maps& maps, const Int4DecodeParams& p, unsign
 
 }  // namespace
 
-cudaError_t launch_paged_decode_int4(const Int4Maps& maps, const Int4DecodeParams& p, int dtype,
-                                     cudaStream_t stream) {
+cudaError_t launch_paged_decode_int4(const Int4DecodeParams& p, int dtype, cudaStream_t stream) {
   const int64_t grid = (int64_t)p.num_seqs * p.num_kv_heads * p.num_parts;
   if (grid > 0x7fffffff || (int64_t)p.num_seqs * p.num_q_heads > 0x7fffffff)
     return cudaErrorInvalidConfiguration;
   const bool wide = p.group > 8;
   if (dtype == B200_DTYPE_BFLOAT16)
-    return wide ? launch_typed<__nv_bfloat16, 2>(maps, p, (unsigned)grid, stream)
-                : launch_typed<__nv_bfloat16, 1>(maps, p, (unsigned)grid, stream);
-  return wide ? launch_typed<__half, 2>(maps, p, (unsigned)grid, stream)
-              : launch_typed<__half, 1>(maps, p, (unsigned)grid, stream);
+    return wide ? launch_typed<__nv_bfloat16, 2>(p, (unsigned)grid, stream)
+                : launch_typed<__nv_bfloat16, 1>(p, (unsigned)grid, stream);
+  return wide ? launch_typed<__half, 2>(p, (unsigned)grid, stream)
+              : launch_typed<__half, 1>(p, (unsigned)grid, stream);
 }
 
 }  // namespace b200
