@@ -380,7 +380,7 @@ typedef struct b200_int4_cache {
   int64_t num_blocks;
   int32_t block_size;   /* multiple of 16 */
   int32_t num_kv_heads;
-  int64_t block_stride_bytes; /* >= block_size * num_kv_heads * 72, multiple of 16 */
+  int64_t block_stride_bytes; /* >= block_size * num_kv_heads * 72, multiple of 128 */
 } b200_int4_cache;
 
 /*
@@ -410,7 +410,16 @@ B200_API int b200_load_kvcache_int4(const b200_int4_cache* cache, const void* sl
                                     int64_t value_row_stride, int32_t dtype,
                                     int32_t* status, void* stream);
 
-/* b200_paged_decode_plan for a 4-bit cache (head_dim 128). */
+/*
+ * Plan of b200_paged_decode_int4. The batch's 32-token tiles are dealt to
+ * num_parts CTAs in equal shares on the device, from the lengths it finds
+ * there: max_kv_len and total_kv_tokens (0 = unknown) only bound the number of
+ * CTAs, and a plan serves every batch of its num_seqs and heads, of whatever
+ * lengths (a captured graph's, for one). part_tokens is 32, or 0 where one CTA
+ * takes each (sequence, KV head) whole: short sequences (max_kv_len up to 512) of
+ * small batches. workspace_bytes is never 0. force_num_parts > 0 sets the number
+ * of CTAs that share.
+ */
 B200_API int b200_paged_decode_int4_plan(int32_t num_seqs, int32_t num_q_heads,
                                          int32_t num_kv_heads, int32_t block_size,
                                          int32_t max_kv_len, int64_t total_kv_tokens,
@@ -420,8 +429,11 @@ B200_API int b200_paged_decode_int4_plan(int32_t num_seqs, int32_t num_q_heads,
  * b200_paged_decode over a 4-bit cache; q and out are `dtype`. max_blocks is
  * the number of valid columns of block_tables: a token past them, or a page id
  * outside the pool, counts as a row of zeros and sets
- * B200_STATUS_PAGE_OUT_OF_RANGE. A sequence of length 0 gives zeros. The kernel
- * is a programmatic dependent of the kernel before it on `stream`, as
+ * B200_STATUS_PAGE_OUT_OF_RANGE. A sequence of length 0 gives zeros. `plan` is
+ * one of b200_paged_decode_int4_plan and the workspace its workspace_bytes of
+ * device memory, 256-byte aligned, whose contents mean nothing between calls;
+ * calls that share one must not overlap on the GPU. The kernel is a
+ * programmatic dependent of the kernel before it on `stream`, as
  * b200_paged_decode is, but reads nothing before that kernel has completed.
  */
 B200_API int b200_paged_decode_int4(const void* q, int64_t q_seq_stride, int64_t q_head_stride,

@@ -684,10 +684,12 @@ int validate_int4_cache(const b200_int4_cache* c, b200::Int4Cache* out) {
   if (((reinterpret_cast<uintptr_t>(c->k_cache) | reinterpret_cast<uintptr_t>(c->v_cache)) & 15) !=
       0)
     return fail(B200_ERR_INVALID_ARGUMENT, "cache base pointers must be 16-byte aligned");
-  if (c->block_stride_bytes % 16 ||
+  if (c->block_stride_bytes % 128 ||
       c->block_stride_bytes < (int64_t)c->block_size * c->num_kv_heads * b200::kInt4RowBytes)
     return fail(B200_ERR_INVALID_ARGUMENT,
-                "block stride must cover a page and be a multiple of 16 bytes");
+                "block stride must cover a page and be a multiple of 128 bytes");
+  if (c->block_stride_bytes > (int64_t(1) << 38) / c->num_blocks)
+    return fail(B200_ERR_UNSUPPORTED, "a cache tensor must not span more than 256 GiB");
   out->k = static_cast<uint8_t*>(c->k_cache);
   out->v = static_cast<uint8_t*>(c->v_cache);
   out->block_stride = c->block_stride_bytes;
@@ -763,6 +765,25 @@ int int4_maps(const b200::Int4Cache& c, int rows, b200::Int4Maps* maps) {
   return int4_tensor_map(c.v, c, true, rows, &maps->vs);
 }
 
+// Decode over a 4-bit cache: units of a KV head's q heads, and the workspace:
+// rows of O of two parts per CTA, where the parts of each (sequence, unit) are,
+// the parts' log2-sum-exp.
+struct Int4Units {
+  int splits, heads;
+};
+Int4Units int4_units(int group) {
+  const int splits = group > b200::kInt4DecodeHeads ? 2 : 1;
+  return {splits, (group + splits - 1) / splits};
+}
+
+int64_t int4_workspace_bytes(int64_t num_seqs, int num_q_heads, int num_kv_heads, int64_t parts) {
+  const Int4Units u = int4_units(num_q_heads / num_kv_heads);
+  const int64_t rows = 2 * parts * u.heads;
+  const int64_t bytes =
+      rows * b200::kHeadDim * 4 + num_seqs * num_kv_heads * u.splits * 16 + rows * 4;
+  return (bytes + 255) / 256 * 256;
+}
+
 int validate_int4_dtype(int32_t dtype) {
   if (dtype != B200_DTYPE_BFLOAT16 && dtype != B200_DTYPE_FLOAT16)
     return fail(B200_ERR_UNSUPPORTED, "dtype must be float16 or bfloat16");
@@ -834,8 +855,33 @@ int b200_load_kvcache_int4(const b200_int4_cache* cache, const void* slot_mappin
 int b200_paged_decode_int4_plan(int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads,
                                 int32_t block_size, int32_t max_kv_len, int64_t total_kv_tokens,
                                 int32_t force_num_parts, b200_decode_plan* plan) {
-  return b200_paged_decode_plan(num_seqs, num_q_heads, num_kv_heads, b200::kHeadDim, block_size,
-                                max_kv_len, total_kv_tokens, force_num_parts, 1, plan);
+  g_last_error.clear();
+  if (plan == nullptr) return fail(B200_ERR_INVALID_ARGUMENT, "plan is NULL");
+  if (num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || max_kv_len <= 0)
+    return fail(B200_ERR_INVALID_ARGUMENT, "sizes must be positive");
+  if (block_size <= 0 || block_size % b200::kTileTokens)
+    return fail(B200_ERR_UNSUPPORTED, "block_size must be a positive multiple of 16");
+  if (num_q_heads % num_kv_heads)
+    return fail(B200_ERR_INVALID_ARGUMENT, "num_q_heads must be divisible by num_kv_heads");
+  if (num_q_heads / num_kv_heads > 16)
+    return fail(B200_ERR_UNSUPPORTED, "at most 16 q heads per KV head");
+  // every CTA that the SMs hold at once, but no more than have work: the
+  // sequences' tiles, of which each has one that may be a rest
+  int64_t tokens = (int64_t)num_seqs * max_kv_len;
+  if (total_kv_tokens > 0 && total_kv_tokens < tokens) tokens = total_kv_tokens;
+  const int64_t tiles = (tokens / b200::kInt4DecodeTile + num_seqs) * num_kv_heads *
+                        int4_units(num_q_heads / num_kv_heads).splits;
+  int64_t parts = b200::int4_decode_ctas(tiles, sm_count());
+  if (force_num_parts > 0) parts = force_num_parts;
+  const int64_t units = (int64_t)num_seqs * num_kv_heads * int4_units(num_q_heads / num_kv_heads).splits;
+  const bool whole =
+      force_num_parts <= 0 &&
+      b200::int4_decode_whole(units, (max_kv_len - 1) / b200::kInt4DecodeTile + 1, sm_count());
+  if (whole) parts = 1;
+  plan->num_parts = static_cast<int32_t>(parts);
+  plan->part_tokens = whole ? 0 : b200::kInt4DecodeTile;
+  plan->workspace_bytes = int4_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, parts);
+  return B200_OK;
 }
 
 int b200_paged_decode_int4(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
@@ -858,20 +904,20 @@ int b200_paged_decode_int4(const void* q, int64_t q_seq_stride, int64_t q_head_s
     return fail(B200_ERR_INVALID_ARGUMENT, "num_q_heads must be divisible by num_kv_heads");
   const int group = num_q_heads / c.num_kv_heads;
   if (group > 16) return fail(B200_ERR_UNSUPPORTED, "at most 16 q heads per KV head");
-  if (plan->num_parts < 1 || plan->part_tokens <= 0 || plan->part_tokens % b200::kTileTokens ||
-      plan->part_tokens > b200::kMaxPartTokens)
-    return fail(B200_ERR_INVALID_ARGUMENT, "malformed decode plan");
+  if (plan->num_parts < 1 ||
+      (plan->part_tokens != b200::kInt4DecodeTile && plan->part_tokens != 0))
+    return fail(B200_ERR_INVALID_ARGUMENT, "the decode plan is not one for a 4-bit cache");
   if (num_seqs == 0) return B200_OK;
   if (!q || !out || !block_tables || !seq_lens)
     return fail(B200_ERR_INVALID_ARGUMENT, "NULL tensor pointer");
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 3) ||
       (q_seq_stride | q_head_stride | out_seq_stride | out_head_stride) & 1)
     return fail(B200_ERR_INVALID_ARGUMENT, "q/out must be 4-byte aligned with even strides");
-  const int64_t need = decode_workspace_bytes(num_seqs, num_q_heads, plan->num_parts);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+  const int64_t need = int4_workspace_bytes(num_seqs, num_q_heads, c.num_kv_heads, plan->num_parts);
+  if (workspace == nullptr || workspace_bytes < need)
     return fail(B200_ERR_INVALID_ARGUMENT,
                 "decode workspace too small: need " + std::to_string(need) + " bytes");
-  if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 255))
+  if (reinterpret_cast<uintptr_t>(workspace) & 255)
     return fail(B200_ERR_INVALID_ARGUMENT, "decode workspace must be 256-byte aligned");
   b200::Int4DecodeParams p{};
   p.q = q;
@@ -884,18 +930,22 @@ int b200_paged_decode_int4(const void* q, int64_t q_seq_stride, int64_t q_head_s
   p.out = out;
   p.out_seq_stride = out_seq_stride;
   p.out_head_stride = out_head_stride;
-  const int64_t slots = (int64_t)num_seqs * num_q_heads * plan->num_parts;
-  p.part_o = need > 0 ? static_cast<float*>(workspace) : nullptr;
-  p.part_lse = need > 0 ? reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                                   (slots * b200::kHeadDim * 4 + 255) / 256 * 256)
-                        : nullptr;
-  p.num_parts = plan->num_parts;
-  p.part_tokens = plan->part_tokens;
-  p.block_size = c.block_size;
+  const Int4Units u = int4_units(group);
   p.group = group;
+  p.splits = u.splits;
+  p.heads = u.heads;
+  p.num_units = c.num_kv_heads * u.splits;
+  char* ws = static_cast<char*>(workspace);
+  p.part_o = reinterpret_cast<float*>(ws);
+  ws += (int64_t)2 * plan->num_parts * u.heads * b200::kHeadDim * 4;
+  p.parts = reinterpret_cast<int4*>(ws);
+  ws += (int64_t)num_seqs * p.num_units * 16;
+  p.part_lse = reinterpret_cast<float*>(ws);
+  p.num_parts = plan->num_parts;
+  p.whole = plan->part_tokens == 0 ? 1 : 0;
+  p.block_size = c.block_size;
   p.num_seqs = num_seqs;
   p.num_q_heads = num_q_heads;
-  p.num_kv_heads = c.num_kv_heads;
   p.cache = c;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.status = status;

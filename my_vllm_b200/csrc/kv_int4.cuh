@@ -31,7 +31,7 @@ constexpr int kInt4RowBytes = kInt4CodeBytes + kInt4ScaleBytes;
 struct Int4Cache {
   uint8_t* k;
   uint8_t* v;
-  int64_t block_stride;  // bytes between consecutive pages
+  int64_t block_stride;  // bytes between consecutive pages, a multiple of 128
   int64_t num_blocks;
   int block_size;
   int num_kv_heads;
@@ -65,20 +65,27 @@ struct Int4DecodeParams {
   void* out;
   int64_t out_seq_stride;
   int64_t out_head_stride;
-  float* part_o;    // [num_seqs, num_q_heads, num_parts, head_dim]
-  float* part_lse;  // [num_seqs, num_q_heads, num_parts], log2 domain
-  int num_parts;
-  int part_tokens;
+  float* part_o;    // [2 num_parts, heads, head_dim]
+  float* part_lse;  // [2 num_parts, heads], log2 domain
+  int4* parts;      // [num_seqs, num_units]: where the parts of each are
+  int num_parts;    // CTAs that share the batch
+  int whole;        // instead a CTA for each (sequence, unit), nothing to join
   int block_size;
-  int group;
   int num_seqs;
   int num_q_heads;
-  int num_kv_heads;
+  int group;      // q heads per KV head
+  int splits;     // units of a KV head: 1, or 2 for groups of more than 8 heads
+  int heads;      // q heads of a unit (the second may have one less)
+  int num_units;  // num_kv_heads * splits
   Int4Cache cache;
   float scale_log2;
   int32_t* status;
 };
 
 cudaError_t launch_paged_decode_int4(const Int4DecodeParams& p, int dtype, cudaStream_t stream);
+constexpr int kInt4DecodeTile = 32;   // tokens
+constexpr int kInt4DecodeHeads = 8;   // q heads of a unit at most
+int64_t int4_decode_ctas(int64_t tiles, int sms);  // that so many tiles are worth
+bool int4_decode_whole(int64_t units, int64_t max_tiles, int sms);
 
 }  // namespace b200

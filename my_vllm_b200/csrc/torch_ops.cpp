@@ -398,13 +398,13 @@ void require_int4_decode(const at::Tensor& q, const at::Tensor& k_cache, const a
   require_int4_attention(q, k_cache, v_cache, out, block_tables, seq_lens, status);
   TORCH_CHECK_VALUE(block_tables.size(0) >= q.size(0) && seq_lens.numel() >= q.size(0),
                     "block_tables / seq_lens must have one row per sequence");
-  TORCH_CHECK_VALUE(num_parts >= 1 && num_parts <= INT32_MAX && part_tokens >= 1 &&
+  TORCH_CHECK_VALUE(num_parts >= 1 && num_parts <= INT32_MAX && part_tokens >= 0 &&
                         part_tokens <= INT32_MAX,
                     "malformed decode plan");
   TORCH_CHECK_VALUE(!workspace.has_value() || workspace->is_contiguous(),
                     "workspace must be contiguous");
-  TORCH_CHECK_VALUE(num_parts == 1 || q.size(0) == 0 || workspace.has_value(),
-                    "decode workspace smaller than the plan requires");
+  TORCH_CHECK_VALUE(q.size(0) == 0 || workspace.has_value(),
+                    "decode over a 4-bit cache needs the plan's workspace");
 }
 
 void paged_decode_int4(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,

@@ -142,10 +142,10 @@ def test_attention_refusals(fake):
     cache = fake(8, 16, 2, 72, dtype=torch.uint8)
     q, out = fake(3, 8, 128), fake(3, 8, 128)
     tables, lens, starts = _i32(fake, 3, 2), _i32(fake, 3), _i32(fake, 4)
-    plan = ops.DecodePlan(1, 32, 0)
+    plan, room = ops.DecodePlan(1, 32, 8192), fake(8192, dtype=torch.uint8)
 
-    def decode(q=q, cache=cache, out=out, plan=plan, **more):
-        return ops.paged_decode(q, cache, cache, tables, lens, out, plan, 0.1, **more)
+    def decode(q=q, cache=cache, out=out, workspace=room, **more):
+        return ops.paged_decode(q, cache, cache, tables, lens, out, plan, 0.1, workspace, **more)
 
     def prefill(q=q, cache=cache, out=out, **more):
         return ops.paged_prefill(q, cache, cache, tables, lens, starts, out, 1, 0.1, **more)
@@ -165,14 +165,26 @@ def test_attention_refusals(fake):
         with pytest.raises(ValueError, match="FP8"):
             call(k_scale=fake(1, dtype=torch.float32))
     with pytest.raises(ValueError, match="workspace"):
-        decode(plan=ops.DecodePlan(2, 16, 4096))
+        decode(workspace=None)
+    with pytest.raises(ValueError, match="contiguous"):
+        decode(workspace=fake(16384, dtype=torch.uint8)[::2])
 
 
 def test_plan_for_a_4bit_cache():
+    # CTAs that share the batch: three per SM of 148, fewer where each would have
+    # under four tiles of 32 tokens (groups of more than 8 heads read theirs twice)
     plan = ops.plan_decode(4, 32, 8, 128, 16, 32768, kv_int4=True)
-    assert plan.num_parts > 1 and plan.num_parts * plan.part_tokens >= 32768
-    assert plan.part_tokens % 16 == 0 and plan.part_tokens <= 8192
-    assert plan.workspace_bytes >= 4 * 32 * plan.num_parts * 129 * 4
+    assert plan.num_parts == 444 and plan.part_tokens == 32
+    assert plan.workspace_bytes >= 2 * 444 * 4 * 129 * 4 + 32 * 16
+    assert ops.plan_decode(1, 16, 1, 128, 16, 640, kv_int4=True).num_parts == 10
+    # up to 512 tokens a sequence, in one wave: nothing is cut (part_tokens 0)
+    for batch, tokens in ((1, 1), (55, 512)):
+        plan = ops.plan_decode(batch, 8, 8, 128, 16, tokens, kv_int4=True)
+        assert (plan.num_parts, plan.part_tokens) == (1, 0)
+    for batch, tokens in ((56, 512), (55, 513)):
+        assert ops.plan_decode(batch, 8, 8, 128, 16, tokens, kv_int4=True).part_tokens == 32
+    assert ops.plan_decode(9, 8, 1, 128, 16, 32768, total_kv_tokens=6400,
+                           kv_int4=True).num_parts == 52
     assert ops.plan_decode(4, 8, 2, 128, 16, 1000, force_num_parts=5, kv_int4=True).num_parts == 5
     with pytest.raises(ValueError, match="either"):
         ops.plan_decode(4, 8, 2, 128, 16, 1000, kv_int4=True, kv_fp8=True)
@@ -182,6 +194,8 @@ def test_plan_for_a_4bit_cache():
         ops.plan_decode(4, 8, 2, 128, 8, 1000, kv_int4=True)
     with pytest.raises(ValueError, match="divisible"):
         ops.plan_decode(4, 9, 2, 128, 16, 1000, kv_int4=True)
+    with pytest.raises(RuntimeError, match="16 q heads"):
+        ops.plan_decode(4, 34, 2, 128, 16, 1000, kv_int4=True)
 
 
 BF16 = _native.DTYPE_BFLOAT16
@@ -202,21 +216,23 @@ BAD_CACHES = [
     (dict(block_size=24), _native.B200_ERR_UNSUPPORTED, b"multiple of 16"),
     (dict(num_kv_heads=0), _native.B200_ERR_INVALID_ARGUMENT, b"positive"),
     (dict(block_stride_bytes=16 * 2 * 72 - 16), _native.B200_ERR_INVALID_ARGUMENT, b"cover"),
-    (dict(block_stride_bytes=16 * 2 * 72 + 8), _native.B200_ERR_INVALID_ARGUMENT, b"16 bytes"),
+    (dict(block_stride_bytes=16 * 2 * 72 + 64), _native.B200_ERR_INVALID_ARGUMENT, b"128 bytes"),
+    (dict(block_stride_bytes=1 << 35), _native.B200_ERR_UNSUPPORTED, b"256 GiB"),
 ]
 
 
 @pytest.mark.parametrize("change,code,text", BAD_CACHES)
 def test_c_abi_refuses_bad_caches(change, code, text):
     lib, bad = _native.load_library(), _cache(**change)
-    plan = _native.DecodePlan(1, 512, 0)
+    plan = _native.DecodePlan(1, 32, 0)
     calls = (
         lambda: lib.b200_store_kvcache_int4(0x3000, 256, 0x4000, 256, BF16, bad, 0x5000, 0, 4,
                                             None, None),
         lambda: lib.b200_load_kvcache_int4(bad, 0x5000, 0, 4, 0x3000, 256, 0x4000, 256, BF16,
                                            None, None),
         lambda: lib.b200_paged_decode_int4(0x3000, 1024, 128, BF16, bad, 0x4000, 8, 8, 0x5000, 4,
-                                           8, 0x6000, 1024, 128, 0.1, plan, None, 0, None, None),
+                                           8, 0x6000, 1024, 128, 0.1, plan, 0x8000, 1 << 20, None,
+                                           None),
         lambda: lib.b200_paged_prefill_int4(0x3000, 1024, 128, BF16, bad, 0x4000, 8, 8, 0x5000,
                                             0x7000, 4, 8, 2, 8, 0x6000, 1024, 128, 0.1, None,
                                             None),
@@ -241,7 +257,7 @@ def test_c_abi_refuses_bad_rows_and_sizes():
     assert store(slots=None) == _native.B200_ERR_INVALID_ARGUMENT
     assert store(n=0, key=None) == _native.B200_OK
 
-    def decode(hq=8, q=0x3000, plan=_native.DecodePlan(1, 512, 0), ws=None, nbytes=0, n=4):
+    def decode(hq=8, q=0x3000, plan=_native.DecodePlan(2, 32, 0), ws=0x8000, nbytes=1 << 20, n=4):
         return lib.b200_paged_decode_int4(q, 1024, 128, BF16, c, 0x4000, 8, 8, 0x5000, n, hq,
                                           0x6000, 1024, 128, 0.1, plan, ws, nbytes, None, None)
 
@@ -250,12 +266,13 @@ def test_c_abi_refuses_bad_rows_and_sizes():
     assert decode(q=0x3002) == _native.B200_ERR_INVALID_ARGUMENT
     assert decode(q=None) == _native.B200_ERR_INVALID_ARGUMENT
     assert decode(plan=None) == _native.B200_ERR_INVALID_ARGUMENT
-    assert decode(plan=_native.DecodePlan(1, 24, 0)) == _native.B200_ERR_INVALID_ARGUMENT
-    assert decode(plan=_native.DecodePlan(1, 16384, 0)) == _native.B200_ERR_INVALID_ARGUMENT
-    split = _native.DecodePlan(4, 512, 0)
-    assert decode(plan=split) == _native.B200_ERR_INVALID_ARGUMENT
+    for bad in (_native.DecodePlan(0, 32, 0), _native.DecodePlan(1, 4096, 0)):
+        assert decode(plan=bad) == _native.B200_ERR_INVALID_ARGUMENT
+        assert b"4-bit" in lib.b200_last_error()
+    assert decode(ws=None) == _native.B200_ERR_INVALID_ARGUMENT
     assert b"workspace" in lib.b200_last_error()
-    assert decode(plan=split, ws=0x8010, nbytes=1 << 20) == _native.B200_ERR_INVALID_ARGUMENT
+    assert decode(nbytes=4096) == _native.B200_ERR_INVALID_ARGUMENT
+    assert decode(ws=0x8010) == _native.B200_ERR_INVALID_ARGUMENT
     assert decode(n=0, q=None) == _native.B200_OK
 
     def prefill(hq=8, q=0x3000, rows=8, most=2, scale=0.1, n=4):
