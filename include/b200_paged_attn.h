@@ -448,8 +448,14 @@ B200_API int b200_paged_decode_int4(const void* q, int64_t q_seq_stride, int64_t
 
 /*
  * b200_paged_prefill over a 4-bit cache; q and out are `dtype`, max_blocks as
- * above. softmax_scale must be positive. No workspace.
+ * above. softmax_scale must be positive. A query row that sees no token gives
+ * zeros. workspace (optional, NULL = none): workspace_bytes() below of device
+ * memory, 256-byte aligned, whose contents mean nothing between calls; calls
+ * that share one must not overlap on the GPU. With it long units are shared by
+ * several SMs and joined in a fixed order; without it each stays on one SM
+ * (64 new tokens on 8k cached ones: 8 of 148 SMs at work).
  */
+B200_API int64_t b200_paged_prefill_int4_workspace_bytes(void);
 B200_API int b200_paged_prefill_int4(const void* q, int64_t q_token_stride,
                                      int64_t q_head_stride, int32_t dtype,
                                      const b200_int4_cache* cache, const int32_t* block_tables,
@@ -458,7 +464,8 @@ B200_API int b200_paged_prefill_int4(const void* q, int64_t q_token_stride,
                                      int32_t num_seqs, int32_t num_q_tokens, int32_t max_q_len,
                                      int32_t num_q_heads, void* out, int64_t out_token_stride,
                                      int64_t out_head_stride, float softmax_scale,
-                                     int32_t* status, void* stream);
+                                     void* workspace, int64_t workspace_bytes, int32_t* status,
+                                     void* stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

@@ -58,6 +58,7 @@ EXPORTED_SYMBOLS = (
     "b200_paged_decode_int4_plan",
     "b200_paged_decode_int4",
     "b200_paged_prefill_int4",
+    "b200_paged_prefill_int4_workspace_bytes",
 )
 
 
@@ -188,10 +189,11 @@ _SIGNATURES = {
     "b200_paged_prefill_int4": (
         [
             _VP, _I64, _I64, _I32, ctypes.POINTER(Int4Cache), _VP, _I64, _I32, _VP, _VP, _I32,
-            _I32, _I32, _I32, _VP, _I64, _I64, _F32, _VP, _VP,
+            _I32, _I32, _I32, _VP, _I64, _I64, _F32, _VP, _I64, _VP, _VP,
         ],
         _I32,
     ),
+    "b200_paged_prefill_int4_workspace_bytes": ([], _I64),
 }
 
 _lock = threading.Lock()

@@ -28,6 +28,7 @@ SOURCES = (
     "kv_append.cu",
     "kv_int4.cu",
     "paged_decode_int4.cu",
+    "paged_prefill_int4.cu",
     "rope_append.cu",
     "paged_decode.cu",
     "paged_prefill_tc.cu",

@@ -699,72 +699,6 @@ int validate_int4_cache(const b200_int4_cache* c, b200::Int4Cache* out) {
   return B200_OK;
 }
 
-// Tensor map over one 4-bit cache tensor's codes (scales = false) or scales, for
-// boxes of `rows` slots (see b200::Int4Maps). `key.dtype` keeps its keys apart
-// from the other maps'.
-int int4_tensor_map(const uint8_t* base, const b200::Int4Cache& c, bool scales, int rows,
-                    CUtensorMap* out) {
-  MapKey key;
-  std::memset(&key, 0, sizeof(key));
-  key.ptr = reinterpret_cast<uint64_t>(base);
-  key.dims[0] = c.num_kv_heads;
-  key.dims[1] = c.block_size;
-  key.dims[2] = c.num_blocks;
-  key.dims[3] = rows;
-  key.strides[0] = c.block_stride;
-  key.dtype = scales ? 2001 : 2000;
-  {
-    std::lock_guard<std::mutex> lock(g_map_mu);
-    auto it = map_cache().find(key);
-    if (it != map_cache().end()) {
-      *out = it->second;
-      return B200_OK;
-    }
-  }
-  auto fn = encode_fn();
-  if (fn == nullptr)
-    return fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
-  const cuuint64_t heads = c.num_kv_heads, bs = c.block_size, blocks = c.num_blocks;
-  const cuuint64_t stride = c.block_stride;
-  const cuuint32_t one[4] = {1, 1, 1, 1};
-  CUtensorMap m;
-  CUresult r;
-  if (scales) {
-    const cuuint64_t dims[3] = {bs * b200::kInt4ScaleBytes, heads, blocks};
-    const cuuint64_t strides[2] = {bs * b200::kInt4ScaleBytes, stride};
-    const cuuint32_t box[3] = {(cuuint32_t)(rows * b200::kInt4ScaleBytes), 1, 1};
-    r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3,
-           const_cast<uint8_t*>(base) + heads * bs * b200::kInt4CodeBytes, dims, strides, box, one,
-           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  } else {
-    const cuuint64_t dims[4] = {b200::kInt4CodeBytes, bs, heads, blocks};
-    const cuuint64_t strides[3] = {b200::kInt4CodeBytes, bs * b200::kInt4CodeBytes, stride};
-    const cuuint32_t box[4] = {b200::kInt4CodeBytes, (cuuint32_t)rows, 1, 1};
-    r = fn(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, box,
-           one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
-           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  }
-  if (r != CUDA_SUCCESS)
-    return fail(B200_ERR_CUDA, "cuTensorMapEncodeTiled (int4) failed with CUresult " +
-                                   std::to_string(static_cast<int>(r)));
-  {
-    std::lock_guard<std::mutex> lock(g_map_mu);
-    if (map_cache().size() > 4096) map_cache().clear();
-    map_cache().emplace(key, m);
-  }
-  *out = m;
-  return B200_OK;
-}
-
-int int4_maps(const b200::Int4Cache& c, int rows, b200::Int4Maps* maps) {
-  int rc;
-  if ((rc = int4_tensor_map(c.k, c, false, rows, &maps->kc)) != B200_OK) return rc;
-  if ((rc = int4_tensor_map(c.k, c, true, rows, &maps->ks)) != B200_OK) return rc;
-  if ((rc = int4_tensor_map(c.v, c, false, rows, &maps->vc)) != B200_OK) return rc;
-  return int4_tensor_map(c.v, c, true, rows, &maps->vs);
-}
-
 // Decode over a 4-bit cache: units of a KV head's q heads, and the workspace:
 // rows of O of two parts per CTA, where the parts of each (sequence, unit) are,
 // the parts' log2-sum-exp.
@@ -954,6 +888,10 @@ int b200_paged_decode_int4(const void* q, int64_t q_seq_stride, int64_t q_head_s
   return B200_OK;
 }
 
+int64_t b200_paged_prefill_int4_workspace_bytes(void) {
+  return b200::kInt4PrefillWorkspaceBytes;
+}
+
 int b200_paged_prefill_int4(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                             int32_t dtype, const b200_int4_cache* cache,
                             const int32_t* block_tables, int64_t block_table_stride,
@@ -961,7 +899,8 @@ int b200_paged_prefill_int4(const void* q, int64_t q_token_stride, int64_t q_hea
                             const int32_t* query_start_loc, int32_t num_seqs,
                             int32_t num_q_tokens, int32_t max_q_len, int32_t num_q_heads,
                             void* out, int64_t out_token_stride, int64_t out_head_stride,
-                            float softmax_scale, int32_t* status, void* stream) {
+                            float softmax_scale, void* workspace, int64_t workspace_bytes,
+                            int32_t* status, void* stream) {
   g_last_error.clear();
   b200::Int4Cache c;
   int rc = validate_int4_dtype(dtype);
@@ -984,7 +923,18 @@ int b200_paged_prefill_int4(const void* q, int64_t q_token_stride, int64_t q_hea
     return fail(B200_ERR_INVALID_ARGUMENT,
                 "q/out must be 16-byte aligned with strides that are multiples of 8");
   if (max_blocks == 0) return fail(B200_ERR_INVALID_ARGUMENT, "block_tables has no columns");
-  b200::PrefillParams p{};
+  if (workspace) {
+    if (reinterpret_cast<uintptr_t>(workspace) & 255)
+      return fail(B200_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+    if (workspace_bytes < b200::kInt4PrefillWorkspaceBytes)
+      return fail(B200_ERR_INVALID_ARGUMENT,
+                  "workspace smaller than b200_paged_prefill_int4_workspace_bytes()");
+  }
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return cuda_fail(e, "device query");
+  b200::Int4PrefillParams p{};
   p.q = q;
   p.q_token_stride = q_token_stride;
   p.q_head_stride = q_head_stride;
@@ -996,31 +946,26 @@ int b200_paged_prefill_int4(const void* q, int64_t q_token_stride, int64_t q_hea
   p.out = out;
   p.out_token_stride = out_token_stride;
   p.out_head_stride = out_head_stride;
-  p.block_size = c.block_size;
+  p.num_seqs = num_seqs;
   p.group = group;
-  p.num_q_heads = num_q_heads;
-  p.num_blocks = c.num_blocks;
+  p.inv_group = 65535 / group + 1;
+  p.num_ctas = sms < b200::kInt4PrefillCtas ? sms : b200::kInt4PrefillCtas;
+  p.cache = c;
+  p.stride128 = static_cast<uint32_t>(c.block_stride / 128);  // at most 2^31
+  // m = floor(2^(31 + s) / d) + 1 with 2^s >= d: m d - 2^(31 + s) <= d <= 2^s, so
+  // t m / 2^(31 + s) exceeds t / d by less than 1 / d for t < 2^31
+  int s = 4;
+  while ((1 << s) < c.block_size) ++s;
+  p.div_mul = static_cast<uint32_t>((uint64_t(1) << (31 + s)) / c.block_size + 1);
+  p.div_shift = s - 1;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  if (workspace) {
+    p.joins = static_cast<int4*>(workspace);
+    p.records = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
+                                         b200::kInt4PrefillJoinBytes);
+  }
   p.status = status;
-  b200::Int4Maps maps;
-  if ((rc = int4_maps(c, b200::kTileTokens, &maps)) != B200_OK) return rc;
-  // Q and whole output tiles by TMA under the conditions of b200_paged_prefill
-  CUtensorMap mq, mo;
-  std::memset(&mq, 0, sizeof(mq));
-  std::memset(&mo, 0, sizeof(mo));
-  p.q_tma = p.o_tma = 128 % group == 0 ? 1 : 0;
-  if (p.q_tma && q_tensor_map(q, dtype, num_q_heads, num_q_tokens, q_head_stride, q_token_stride,
-                              group, &mq) != B200_OK) {
-    p.q_tma = 0;
-    g_last_error.clear();
-  }
-  if (p.o_tma && q_tensor_map(out, dtype, num_q_heads, num_q_tokens, out_head_stride,
-                              out_token_stride, group, &mo) != B200_OK) {
-    p.o_tma = 0;
-    g_last_error.clear();
-  }
-  cudaError_t e = b200::launch_paged_prefill_int4(maps, mq, mo, p, dtype, c.num_kv_heads, num_seqs,
-                                                  max_q_len, static_cast<cudaStream_t>(stream));
+  e = b200::launch_paged_prefill_int4(p, dtype, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "int4 paged prefill launch");
   return B200_OK;
 }

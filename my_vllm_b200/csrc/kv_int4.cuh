@@ -17,7 +17,6 @@
 // scales, each contiguous, whatever the number of heads.
 #pragma once
 
-#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -46,13 +45,6 @@ cudaError_t launch_load_kvcache_int4(const Int4Cache& cache, const void* slots, 
                                      int64_t num_tokens, void* key, int64_t key_row_stride,
                                      void* value, int64_t value_row_stride, int dtype,
                                      int32_t* status, cudaStream_t stream);
-
-// Tensor maps of a cache pair (built by the C ABI layer). Codes: (byte of a row
-// 64, slot, head, page), box 64 x box_rows x 1 x 1, 64-byte swizzle. Scales:
-// (byte of a head's scales 8 block_size, head, page), box 8 box_rows x 1 x 1.
-struct Int4Maps {
-  CUtensorMap kc, ks, vc, vs;
-};
 
 struct Int4DecodeParams {
   const void* q;
@@ -87,5 +79,36 @@ constexpr int kInt4DecodeTile = 32;   // tokens
 constexpr int kInt4DecodeHeads = 8;   // q heads of a unit at most
 int64_t int4_decode_ctas(int64_t tiles, int sms);  // that so many tiles are worth
 bool int4_decode_whole(int64_t units, int64_t max_tiles, int sms);
+
+struct Int4PrefillParams {
+  const void* q;
+  int64_t q_token_stride;
+  int64_t q_head_stride;
+  const int32_t* block_tables;
+  int64_t block_table_stride;
+  int max_blocks;  // valid columns of block_tables
+  const int32_t* seq_lens;
+  const int32_t* query_start_loc;
+  int num_seqs;
+  void* out;
+  int64_t out_token_stride;
+  int64_t out_head_stride;
+  int group;       // q heads per KV head
+  int inv_group;   // r / group = r * inv_group >> 16, r < 256
+  int num_ctas;
+  Int4Cache cache;
+  uint32_t stride128;           // cache.block_stride / 128
+  uint32_t div_mul, div_shift;  // t / block_size = umulhi(t, div_mul) >> div_shift, t < 2^31
+  float scale_log2;
+  int4* joins;     // [num_ctas]; with records: parts, first query row, rows, KV head
+  float* records;  // [2 num_ctas], or nullptr: no unit is split
+  int32_t* status;
+};
+constexpr int kInt4PrefillCtas = 148;  // at most: one for each SM
+constexpr int64_t kInt4PrefillRecordBytes = 2 * 130 * 128 * 4;
+constexpr int64_t kInt4PrefillJoinBytes = (kInt4PrefillCtas * 16 + 255) / 256 * 256;
+constexpr int64_t kInt4PrefillWorkspaceBytes =
+    kInt4PrefillJoinBytes + 2 * kInt4PrefillCtas * kInt4PrefillRecordBytes;
+cudaError_t launch_paged_prefill_int4(const Int4PrefillParams& p, int dtype, cudaStream_t stream);
 
 }  // namespace b200

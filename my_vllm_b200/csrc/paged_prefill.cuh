@@ -43,7 +43,6 @@ struct PrefillParams {
   int* split_tickets;    // [split_cap][2 Q tiles], zeroed before each launch
   int split_cap;         // part records the workspace holds
   int num_sms;
-  int max_blocks;  // 4-bit caches: valid columns of a block-table row (at least 1)
 };
 
 // Part records of the prefill split-KV workspace and its size.
@@ -65,12 +64,5 @@ cudaError_t launch_paged_prefill_tc(const CUtensorMap& mk, const CUtensorMap& mv
                                     const PrefillParams& p, int dtype, bool kv_fp8,
                                     int num_kv_heads, int num_seqs, int max_q_len,
                                     cudaStream_t stream);
-
-// The same over a 4-bit cache (maps for boxes of 16 slots); no workspace.
-struct Int4Maps;
-cudaError_t launch_paged_prefill_int4(const Int4Maps& maps, const CUtensorMap& mq,
-                                      const CUtensorMap& mo, const PrefillParams& p, int dtype,
-                                      int num_kv_heads, int num_seqs, int max_q_len,
-                                      cudaStream_t stream);
 
 }  // namespace b200

@@ -55,20 +55,12 @@
 //     MMAs run kind::f16 on fp16 operands; the K scale folds into the softmax
 //     scale and the V scale into the final normalisation. The K ring has 2
 //     stages instead of 3 to make room for the staging ring.
-//   * 4-bit caches (kKvInt4, format in kv_int4.cuh) take the FP8 road: a
-//     128-token tile lands as 8 KiB of codes and 1 KiB of scales, and four
-//     converter warps, one on each SM sub-partition, write s (c - 8) rounded
-//     to T, the MMAs' type (bf16 keeps the scales' range, fp16 is exact). A
-//     value group without a finite scale is written as 0 and its first token
-//     remembered per group of 32 columns: rows that see the token get NaN there
-//     in the epilogue, rows before it do not (0 * NaN inside an MMA would spread).
 #include <cuda_runtime.h>
 #include <math.h>
 
 #include <type_traits>
 
 #include "common.cuh"
-#include "kv_int4.cuh"
 #include "paged_decode.cuh"
 #include "paged_prefill.cuh"
 #include "tcgen05.cuh"
@@ -80,30 +72,24 @@ constexpr int kTcTiles = 2;    // Q tiles per CTA
 constexpr int kTcKv = 128;     // KV tokens per tile (N of QK^T, K of PV)
 constexpr int kTcProducerWarp = 8;
 constexpr int kTcMmaWarp = 9;
-// How the cache holds K and V.
-constexpr int kKv16 = 0, kKvFp8 = 1, kKvInt4 = 2;
-constexpr int kTcConvWarp0 = 10;  // FP8: warps 10-11, 4-bit: warps 10-13 convert staged tiles
-template <int kKv>
-constexpr int kTcConvWarps = kKv == kKv16 ? 0 : kKv == kKvFp8 ? 2 : 4;
-template <int kKv>
-constexpr int tc_threads() { return (10 + kTcConvWarps<kKv>) * 32; }
+constexpr int kTcConvWarp0 = 10;  // FP8 only: warps 10 and 11 convert staged tiles
+constexpr int kTcConvWarps = 2;
+template <bool kFp8>
+constexpr int tc_threads() { return (kFp8 ? 12 : 10) * 32; }
 constexpr int kTcHalf = kTcRows * 128;          // [128 rows x 64 elements] = 16 KiB
 constexpr int kTcQ = 0;                         // Q_A, Q_B: 2 x 32 KiB
 constexpr int kTcTileBytes = 2 * kTcHalf;       // one K or V tile (lo/hi halves) = 32 KiB
 constexpr int kTcVStages = 2;                   // V is freed after the PV MMAs
 constexpr int kTcK0 = kTcTiles * kTcTileBytes;
 constexpr int kTcRawTileBytes = kTcKv * 128;    // one FP8 K or V tile = 16 KiB
-constexpr int kTcInt4CodeTile = kTcKv * kInt4CodeBytes;               // 8 KiB
-constexpr int kTcInt4TileBytes = kTcKv * kInt4RowBytes;               // codes + scales = 9 KiB
-// Shared-memory map per cache type: Q_A | Q_B | K ring | V ring | [staging] | barriers.
+// Shared-memory map per cache type: Q_A | Q_B | K ring | V ring | [FP8 staging] | barriers.
 // K is freed after the S MMAs, so a deeper ring lets it run further ahead.
-template <int kKv>
+template <bool kFp8>
 struct TcLayout {
-  static constexpr int kKStages = kKv != kKv16 ? 2 : 3;
+  static constexpr int kKStages = kFp8 ? 2 : 3;
   static constexpr int kV0 = kTcK0 + kKStages * kTcTileBytes;
-  static constexpr int kRaw0 = kV0 + kTcVStages * kTcTileBytes;  // staging, 2 slots
-  static constexpr int kRawBytes = kKv == kKvInt4 ? kTcInt4TileBytes : kTcRawTileBytes;
-  static constexpr int kBars = kRaw0 + (kKv != kKv16 ? 2 * kRawBytes : 0);
+  static constexpr int kRaw0 = kV0 + kTcVStages * kTcTileBytes;  // FP8 staging, 2 slots
+  static constexpr int kBars = kRaw0 + (kFp8 ? 2 * kTcRawTileBytes : 0);
   static constexpr int kSmemBytes = 1024 + kBars + 256;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
@@ -120,55 +106,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ uint32_t pair_to_f16(uint32_t w, __half) { return w; }
 __device__ __forceinline__ uint32_t pair_to_f16(uint32_t w, __nv_bfloat16) {
   return Elem<__half>::pack(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-
-// The scales' tensor maps of a 4-bit cache; nothing for the other types.
-template <int kKv>
-struct TcScaleMaps {};
-template <>
-struct TcScaleMaps<kKvInt4> {
-  CUtensorMap k, v;
-};
-
-// 8 codes of a 4-bit row -> 8 values of T in order, each rn(s (c - 8)).
-struct Int4Scale {
-  uint32_t mul, post;  // pairs
-};
-__device__ __forceinline__ Int4Scale int4_scale(uint32_t bits, __nv_bfloat16) {
-  return {bits | (bits << 16), 0u};
-}
-__device__ __forceinline__ Int4Scale int4_scale(uint32_t bits, __half) {
-  // s below 1 is multiplied in as 256 s, exact where s alone would be subnormal
-  // in fp16; the last product, by 2^-8, then rounds once
-  const float s = __uint_as_float(bits << 16);
-  const bool small = s < 1.f;
-  const float m = small ? s * 256.f : s;
-  return {Elem<__half>::pack(m, m), small ? 0x1c001c00u : 0x3c003c00u};
-}
-__device__ __forceinline__ uint32_t int4_pair(uint32_t codes, const Int4Scale& s, __nv_bfloat16) {
-  uint32_t v = codes | 0x43004300u;  // 128 + c
-  asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(0xc308c308u));  // - 136
-  asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(s.mul));
-  return v;
-}
-__device__ __forceinline__ uint32_t int4_pair(uint32_t codes, const Int4Scale& s, __half) {
-  uint32_t v = codes | 0x64006400u;  // 1024 + c
-  asm("add.rn.f16x2 %0, %0, %1;" : "+r"(v) : "r"(0xe408e408u));  // - 1032
-  asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(v) : "r"(s.mul));
-  asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(v) : "r"(s.post));
-  return v;
-}
-template <typename T>
-__device__ __forceinline__ uint4 int4_values(uint32_t w, const Int4Scale& s) {
-  // byte k of w to the low half, byte k of w >> 4 to the high half: the two
-  // nibbles of a byte, which are neighbours, in their places
-  const uint32_t t = w >> 4;
-  uint4 v;
-  v.x = int4_pair(__byte_perm(w, t, 0x4400) & 0x000f000fu, s, T());
-  v.y = int4_pair(__byte_perm(w, t, 0x5511) & 0x000f000fu, s, T());
-  v.z = int4_pair(__byte_perm(w, t, 0x6622) & 0x000f000fu, s, T());
-  v.w = int4_pair(__byte_perm(w, t, 0x7733) & 0x000f000fu, s, T());
-  return v;
 }
 
 // Work units are (sequence, row block, KV head). A unit's cost is the number
@@ -368,18 +305,14 @@ struct TilePages {
   }
 };
 
-template <typename T, int kKv>
-__global__ void __launch_bounds__(tc_threads<kKv>(), 1)
+template <typename T, bool kFp8>
+__global__ void __launch_bounds__(tc_threads<kFp8>(), 1)
     paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_k,
                             const __grid_constant__ CUtensorMap tmap_v,
                             const __grid_constant__ CUtensorMap tmap_q,
                             const __grid_constant__ CUtensorMap tmap_o,
-                            const __grid_constant__ TcScaleMaps<kKv> tmap_s,
                             const PrefillParams p) {
-  constexpr bool kFp8 = kKv == kKvFp8;
-  constexpr bool kInt4 = kKv == kKvInt4;
-  constexpr int kConvWarps = kTcConvWarps<kKv>;
-  using L = TcLayout<kKv>;
+  using L = TcLayout<kFp8>;
   using M = typename std::conditional<kFp8, __half, T>::type;  // MMA operand type
   constexpr int kTcKStages = L::kKStages;
   constexpr int kTcV0 = L::kV0;
@@ -402,8 +335,6 @@ __global__ void __launch_bounds__(tc_threads<kKv>(), 1)
   uint64_t* p_ready_hi = bars + 23; // [2] per Q tile: P tokens 64-127 written -> MMA
   uint64_t* q_raw = bars + 25;      // FP8 caches: 16-bit Q landed by TMA -> softmax warps
   uint64_t* o_staged = bars + 26;   // [2] per Q tile (128 arrivals): output rows in smem
-  int* nan_token = reinterpret_cast<int*>(bars + 28);  // [4] 4-bit: first token of each value
-                                                       // group without a finite scale
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -416,19 +347,7 @@ __global__ void __launch_bounds__(tc_threads<kKv>(), 1)
   const int group = p.group;
   const int tpc = (kTcTiles * kTcRows) / group;  // query tokens per CTA
   const int tok_begin = rb * tpc;
-  if (tok_begin >= q_len || seq_len <= 0) {  // CTA-uniform, before any sync
-    if (kInt4) {  // rows of a sequence without tokens are zeros
-      const int rows = min(tpc, q_len - tok_begin) * group;
-      for (int i = threadIdx.x; i < rows * 16; i += blockDim.x) {
-        const int r = i >> 4;
-        T* row = reinterpret_cast<T*>(p.out) +
-                 (int64_t)(q_start + tok_begin + r / group) * p.out_token_stride +
-                 (int64_t)(kvh * group + r % group) * p.out_head_stride;
-        reinterpret_cast<uint4*>(row)[i & 15] = make_uint4(0, 0, 0, 0);
-      }
-    }
-    return;
-  }
+  if (tok_begin >= q_len || seq_len <= 0) return;  // CTA-uniform, before any sync
   const int ctx = seq_len - q_len;
 
   // KV tiles each Q tile needs: up to its last valid row's causal limit.
@@ -446,8 +365,8 @@ __global__ void __launch_bounds__(tc_threads<kKv>(), 1)
 
   const uint32_t sbase = smem_u32(smem);
   if (threadIdx.x == 0) {
-    // staged types: a K/V tile is full when every converter warp has written its rows
-    const uint32_t fills = kKv != kKv16 ? kConvWarps : 1;
+    // FP8: a K/V tile is full when both converter warps have written their rows
+    const uint32_t fills = kFp8 ? kTcConvWarps : 1;
     for (int i = 0; i < kTcKStages; ++i) {
       mbar_init(smem_u32(&k_full[i]), fills);
       mbar_init(smem_u32(&k_empty[i]), 1);
@@ -468,14 +387,12 @@ __global__ void __launch_bounds__(tc_threads<kKv>(), 1)
     mbar_init(smem_u32(q_full), (p.q_tma && !kFp8) ? 1 : 2 * kTcRows);
     mbar_init(smem_u32(q_raw), 1);
     for (int x = 0; x < kTcTiles; ++x) mbar_init(smem_u32(&o_staged[x]), kTcRows);
-    if (kKv != kKv16) {
+    if (kFp8) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(smem_u32(&raw_full[i]), 1);
-        mbar_init(smem_u32(&raw_empty[i]), kConvWarps);
+        mbar_init(smem_u32(&raw_empty[i]), kTcConvWarps);
       }
     }
-    if (kInt4)
-      for (int g = 0; g < 4; ++g) nan_token[g] = 0x7fffffff;
     mbar_init_fence();
   }
   if (warp == kTcMmaWarp) {
@@ -544,9 +461,9 @@ __global__ void __launch_bounds__(tc_threads<kKv>(), 1)
   const uint32_t tmem_base = *tmem_slot;
   bool ok = true;
 
-  // Staged items in the 16-bit producer's order: K0, K1, then (V_m, K_{m+2}),
+  // FP8 items in the 16-bit producer's order: K0, K1, then (V_m, K_{m+2}),
   // then the last V tiles. Item i is TMA-loaded into staging slot i % 2 by
-  // the producer warp and converted into its 16-bit K or V stage by warps 10 on.
+  // the producer warp and converted into its fp16 K or V stage by warps 10-11.
   const int k_first = min(2, n_total);
   const int kv_pairs = max(0, n_total - 2);
   auto item_at = [&](int i, bool& is_v, int& j) {
@@ -576,12 +493,11 @@ __global__ void __launch_bounds__(tc_threads<kKv>(), 1)
         tma_load_3d(sbase + kTcQ + x * kTcTileBytes + h * kTcHalf, &tmap_q, smem_u32(bar),
                     h * 64, kvh * group, q_start + tok_begin + x * tpt);
   };
-  if (warp == kTcProducerWarp && kKv != kKv16) {
-    // ---------------------------------------------------- staged producer --
-    if (p.q_tma && lane == 0) load_q(kFp8 ? q_raw : q_full);
+  if (warp == kTcProducerWarp && kFp8) {
+    // ------------------------------------------------------- FP8 producer --
+    if (p.q_tma && lane == 0) load_q(q_raw);
     __syncwarp();
-    const int max_page_idx =
-        kInt4 ? min((seq_len - 1) / p.block_size, p.max_blocks - 1) : (seq_len - 1) / p.block_size;
+    const int max_page_idx = (seq_len - 1) / p.block_size;
     TilePages pages{p.block_tables + (int64_t)s * p.block_table_stride, max_page_idx,
                     p.block_size, lane, 0, 0};
     pages.init();
@@ -600,27 +516,10 @@ __global__ void __launch_bounds__(tc_threads<kKv>(), 1)
       item_at(i, is_v, j);
       if (is_v) pages.advance(j);
       const uint32_t bar = smem_u32(&raw_full[i & 1]);
-      if (lane == 0) mbar_arrive_expect_tx(bar, L::kRawBytes);
+      if (lane == 0) mbar_arrive_expect_tx(bar, kTcRawTileBytes);
       __syncwarp();
-      int page = pages.page(j);
-      if constexpr (kInt4) {
-        if (lane < kTcKv / kTileTokens) {
-          const int tok = j * kTcKv + lane * kTileTokens;
-          const int col = tok / p.block_size;
-          const int row = tok - col * p.block_size;
-          // past the sequence end: zeros; past the table, or outside the pool: zeros and a report
-          if (col > max_page_idx) page = -1;
-          if (page < 0 || page >= p.num_blocks) {
-            if (tok < seq_len) report_status(p.status, B200_STATUS_PAGE_OUT_OF_RANGE);
-            page = -1;
-          }
-          const uint32_t slot = raw0 + (i & 1) * L::kRawBytes;
-          tma_load_4d(slot + lane * (kTileTokens * kInt4CodeBytes), is_v ? &tmap_v : &tmap_k, bar,
-                      0, row, kvh, page);
-          tma_load_3d(slot + kTcInt4CodeTile + lane * (kTileTokens * kInt4ScaleBytes),
-                      is_v ? &tmap_s.v : &tmap_s.k, bar, row * kInt4ScaleBytes, kvh, page);
-        }
-      } else if (lane < kTcKv / kTileTokens) {
+      const int page = pages.page(j);
+      if (lane < kTcKv / kTileTokens) {
         const int tok = j * kTcKv + lane * kTileTokens;
         // past the sequence end: the last page (any valid one), masked later
         const int row = tok / p.block_size > max_page_idx ? 0 : tok % p.block_size;
@@ -636,64 +535,12 @@ __global__ void __launch_bounds__(tc_threads<kKv>(), 1)
       for (int i = max(0, issued - 2); i < issued; ++i)  // loads still in flight
         mbar_wait(smem_u32(&raw_full[i & 1]), (i >> 1) & 1);
     }
-  } else if (kInt4 && warp >= kTcConvWarp0) {
-    // --------------------------------------------- 4-bit converter warps --
-    // Warp 10 + c converts rows 32c .. 32c + 31, 8 rows at a time: lane l holds
-    // row l % 8's 16-byte chunk l / 8, the 32 codes of one scale group, and
-    // writes its 64 bytes of T as four 16-byte chunks of half l / 16 (reads
-    // and writes without bank conflicts under both swizzles).
-    const int row0 = (warp - kTcConvWarp0) * (kTcKv / 4);
-    const int c = lane >> 3;
-    for (int i = 0; i < n_items; ++i) {
-      bool is_v;
-      int j;
-      item_at(i, is_v, j);
-      const int nst = is_v ? kTcVStages : kTcKStages;
-      const int st = j % nst;
-      bool got = true;
-      if (j >= nst)  // the stage is free once the MMAs that read it retired
-        got = mbar_wait(smem_u32(&(is_v ? v_empty : k_empty)[st]), ((j / nst) - 1) & 1);
-      if (got) got = mbar_wait(smem_u32(&raw_full[i & 1]), (i >> 1) & 1);
-      if (!__all_sync(0xffffffffu, got)) {
-        ok = false;
-        break;
-      }
-      const uint8_t* raw = smem + L::kRaw0 + (i & 1) * L::kRawBytes;
-      uint8_t* dst = smem + (is_v ? kTcV0 : kTcK0) + st * kTcTileBytes + (c >> 1) * kTcHalf;
-#pragma unroll 2
-      for (int it = 0; it < 4; ++it) {
-        const int r = row0 + it * 8 + (lane & 7);
-        const uint4 w =
-            *reinterpret_cast<const uint4*>(raw + r * kInt4CodeBytes + ((c ^ ((r >> 1) & 3)) << 4));
-        uint32_t bits =
-            *reinterpret_cast<const uint16_t*>(raw + kTcInt4CodeTile + r * kInt4ScaleBytes + c * 2);
-        if (is_v && bits >= 0x7f80u) {
-          if (j * kTcKv + r < seq_len) atomicMin(&nan_token[c], j * kTcKv + r);
-          bits = 0;
-        }
-        const Int4Scale sc = int4_scale(bits, T());
-        const int c0 = (c & 1) * 4;
-        *reinterpret_cast<uint4*>(dst + swz128(r, c0)) = int4_values<T>(w.x, sc);
-        *reinterpret_cast<uint4*>(dst + swz128(r, c0 + 1)) = int4_values<T>(w.y, sc);
-        *reinterpret_cast<uint4*>(dst + swz128(r, c0 + 2)) = int4_values<T>(w.z, sc);
-        *reinterpret_cast<uint4*>(dst + swz128(r, c0 + 3)) = int4_values<T>(w.w, sc);
-      }
-      // generic-proxy reads of the staging slot and writes of the tile -> async
-      // proxy, then hand off (as the FP8 converters do)
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(smem_u32(&raw_empty[i & 1]));
-        mbar_arrive(smem_u32(is_v ? &v_full[st] : &k_full[st]));
-      }
-    }
-    if (!ok && lane == 0) report_status(p.status, B200_STATUS_WAIT_TIMEOUT);
   } else if (kFp8 && warp >= kTcConvWarp0) {
     // ----------------------------------------------- FP8 converter warps --
     // Warp 10 converts rows 0-63 of every staged tile, warp 11 rows 64-127:
     // chunk c of a row (E4M3 d = 16c .. 16c + 15) -> fp16 chunks 2c', 2c'+1
     // of half c / 4 (c' = c % 4), all 128-byte swizzled like the TMA tiles.
-    const int row0 = (warp - kTcConvWarp0) * (kTcKv / 2);
+    const int row0 = (warp - kTcConvWarp0) * (kTcKv / kTcConvWarps);
     const int c = lane & 7;
     const int h = c >> 2;
     const int c2 = (c & 3) * 2;
@@ -714,7 +561,7 @@ __global__ void __launch_bounds__(tc_threads<kKv>(), 1)
       const uint8_t* raw = smem + L::kRaw0 + (i & 1) * kTcRawTileBytes;
       uint8_t* dst = smem + (is_v ? kTcV0 : kTcK0) + st * kTcTileBytes + h * kTcHalf;
 #pragma unroll 4
-      for (int it = 0; it < kTcKv / 2 / 4; ++it) {
+      for (int it = 0; it < kTcKv / kTcConvWarps / 4; ++it) {
         const int r = row0 + it * 4 + (lane >> 3);
         const uint4 w = *reinterpret_cast<const uint4*>(raw + swz128(r, c));
         uint4 lo, hi;
@@ -1026,15 +873,13 @@ __global__ void __launch_bounds__(tc_threads<kKv>(), 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const float* ov = reinterpret_cast<const float*>(ob[c]);
-          float inv = inv_l;
-          if (kInt4 && qpos >= nan_token[c]) inv = __uint_as_float(0x7fc00000u);
 #pragma unroll
           for (int q8 = 0; q8 < 4; ++q8) {
             uint4 pk;
-            pk.x = pack2<T>(ov[q8 * 8 + 0] * inv, ov[q8 * 8 + 1] * inv);
-            pk.y = pack2<T>(ov[q8 * 8 + 2] * inv, ov[q8 * 8 + 3] * inv);
-            pk.z = pack2<T>(ov[q8 * 8 + 4] * inv, ov[q8 * 8 + 5] * inv);
-            pk.w = pack2<T>(ov[q8 * 8 + 6] * inv, ov[q8 * 8 + 7] * inv);
+            pk.x = pack2<T>(ov[q8 * 8 + 0] * inv_l, ov[q8 * 8 + 1] * inv_l);
+            pk.y = pack2<T>(ov[q8 * 8 + 2] * inv_l, ov[q8 * 8 + 3] * inv_l);
+            pk.z = pack2<T>(ov[q8 * 8 + 4] * inv_l, ov[q8 * 8 + 5] * inv_l);
+            pk.w = pack2<T>(ov[q8 * 8 + 6] * inv_l, ov[q8 * 8 + 7] * inv_l);
             const int chunk = c * 4 + q8;  // 16-byte chunk of the 256-byte row
             if (box_out)
               *reinterpret_cast<uint4*>(otile + (chunk >> 3) * kTcHalf + swz128(t, chunk & 7)) = pk;
@@ -1096,7 +941,7 @@ constexpr int kTcMaxUnitsPerCta = 64;
 // streaming of every SM one such round trip took microseconds)
 constexpr int kTcUnitInts = 6;
 constexpr int kTcPersistSmem =
-    TcLayout<kKv16>::kSmemBytes + kTcMaxUnitsPerCta * kTcUnitInts * 4;  // + the unit list
+    TcLayout<false>::kSmemBytes + kTcMaxUnitsPerCta * kTcUnitInts * 4;  // + the unit list
 static_assert(kTcPersistSmem <= 227 * 1024, "shared memory budget");
 // Split-KV: a unit of more than twice the launch's average work per SM is cut
 // into at most kTcMaxParts KV parts of at least kTcMinPartTiles tiles each
@@ -1352,12 +1197,12 @@ __device__ __forceinline__ TcUnit tc_unit(const PrefillParams& p, const int* e) 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(tc_threads<kKv16>(), 1)
+__global__ void __launch_bounds__(tc_threads<false>(), 1)
     paged_prefill_tc_persistent_kernel(const __grid_constant__ CUtensorMap tmap_k,
                                        const __grid_constant__ CUtensorMap tmap_v,
                                        const __grid_constant__ CUtensorMap tmap_q,
                                        const PrefillParams p) {
-  using L = TcLayout<kKv16>;
+  using L = TcLayout<false>;
   constexpr int kKSt = L::kKStages;
   constexpr int kTcV0 = L::kV0;
   extern __shared__ uint8_t smem_raw[];
@@ -2074,14 +1919,13 @@ __global__ void __launch_bounds__(tc_threads<kKv16>(), 1)
   }
 }
 
-template <typename T, int kKv>
+template <typename T, bool kFp8>
 static cudaError_t launch_tc_typed(const CUtensorMap& mk, const CUtensorMap& mv,
                                    const CUtensorMap& mq, const CUtensorMap& mo,
-                                   const TcScaleMaps<kKv>& ms, const PrefillParams& p,
-                                   int num_kv_heads, int num_seqs, int max_q_len,
-                                   cudaStream_t stream) {
-  auto kernel = paged_prefill_tc_kernel<T, kKv>;
-  constexpr int kSmem = TcLayout<kKv>::kSmemBytes;
+                                   const PrefillParams& p, int num_kv_heads, int num_seqs,
+                                   int max_q_len, cudaStream_t stream) {
+  auto kernel = paged_prefill_tc_kernel<T, kFp8>;
+  constexpr int kSmem = TcLayout<kFp8>::kSmemBytes;
   cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kernel), kSmem);
   if (e != cudaSuccess) return e;
   const int tpc = (kTcTiles * kTcRows) / p.group;
@@ -2093,7 +1937,7 @@ static cudaError_t launch_tc_typed(const CUtensorMap& mk, const CUtensorMap& mv,
   q.blocks_per_seq = blocks;
   const int64_t units = (int64_t)blocks * num_kv_heads * num_seqs;
   if (units > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  if constexpr (kKv == kKv16) {
+  if constexpr (!kFp8) {
     int dev = 0, sms = 0;
     if (q.q_tma) {
       if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
@@ -2120,11 +1964,11 @@ static cudaError_t launch_tc_typed(const CUtensorMap& mk, const CUtensorMap& mv,
       int64_t grid = items < sms ? items : sms;
       const int64_t min_grid = (items + kTcMaxUnitsPerCta - 1) / kTcMaxUnitsPerCta;
       if (grid < min_grid) grid = min_grid;
-      pkernel<<<(unsigned)grid, tc_threads<kKv16>(), kTcPersistSmem, stream>>>(mk, mv, mq, q);
+      pkernel<<<(unsigned)grid, tc_threads<false>(), kTcPersistSmem, stream>>>(mk, mv, mq, q);
       return cudaGetLastError();
     }
   }
-  kernel<<<(unsigned)units, tc_threads<kKv>(), kSmem, stream>>>(mk, mv, mq, mo, ms, q);
+  kernel<<<(unsigned)units, tc_threads<kFp8>(), kSmem, stream>>>(mk, mv, mq, mo, q);
   return cudaGetLastError();
 }
 
@@ -2133,29 +1977,15 @@ cudaError_t launch_paged_prefill_tc(const CUtensorMap& mk, const CUtensorMap& mv
                                     const PrefillParams& p, int dtype, bool kv_fp8,
                                     int num_kv_heads, int num_seqs, int max_q_len,
                                     cudaStream_t stream) {
-  const TcScaleMaps<kKv16> m16{};
-  const TcScaleMaps<kKvFp8> m8{};
   if (dtype == B200_DTYPE_BFLOAT16)
-    return kv_fp8 ? launch_tc_typed<__nv_bfloat16, kKvFp8>(mk, mv, mq, mo, m8, p, num_kv_heads,
-                                                           num_seqs, max_q_len, stream)
-                  : launch_tc_typed<__nv_bfloat16, kKv16>(mk, mv, mq, mo, m16, p, num_kv_heads,
-                                                          num_seqs, max_q_len, stream);
-  return kv_fp8 ? launch_tc_typed<__half, kKvFp8>(mk, mv, mq, mo, m8, p, num_kv_heads, num_seqs,
-                                                  max_q_len, stream)
-                : launch_tc_typed<__half, kKv16>(mk, mv, mq, mo, m16, p, num_kv_heads, num_seqs,
-                                                 max_q_len, stream);
-}
-
-cudaError_t launch_paged_prefill_int4(const Int4Maps& maps, const CUtensorMap& mq,
-                                      const CUtensorMap& mo, const PrefillParams& p, int dtype,
-                                      int num_kv_heads, int num_seqs, int max_q_len,
-                                      cudaStream_t stream) {
-  const TcScaleMaps<kKvInt4> ms{maps.ks, maps.vs};
-  return dtype == B200_DTYPE_BFLOAT16
-             ? launch_tc_typed<__nv_bfloat16, kKvInt4>(maps.kc, maps.vc, mq, mo, ms, p,
-                                                       num_kv_heads, num_seqs, max_q_len, stream)
-             : launch_tc_typed<__half, kKvInt4>(maps.kc, maps.vc, mq, mo, ms, p, num_kv_heads,
-                                                num_seqs, max_q_len, stream);
+    return kv_fp8 ? launch_tc_typed<__nv_bfloat16, true>(mk, mv, mq, mo, p, num_kv_heads, num_seqs,
+                                                         max_q_len, stream)
+                  : launch_tc_typed<__nv_bfloat16, false>(mk, mv, mq, mo, p, num_kv_heads, num_seqs,
+                                                          max_q_len, stream);
+  return kv_fp8 ? launch_tc_typed<__half, true>(mk, mv, mq, mo, p, num_kv_heads, num_seqs, max_q_len,
+                                                stream)
+                : launch_tc_typed<__half, false>(mk, mv, mq, mo, p, num_kv_heads, num_seqs, max_q_len,
+                                                 stream);
 }
 
 }  // namespace b200

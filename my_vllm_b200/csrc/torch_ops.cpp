@@ -440,9 +440,10 @@ void require_int4_prefill(const at::Tensor& q, const at::Tensor& k_cache,
                           const at::Tensor& v_cache, const at::Tensor& block_tables,
                           const at::Tensor& seq_lens, const at::Tensor& query_start_loc,
                           const at::Tensor& out, int64_t max_q_len, int64_t num_seqs,
-                          const std::optional<at::Tensor>& status) {
+                          const std::optional<at::Tensor>& status,
+                          const std::optional<at::Tensor>& workspace) {
   require_one_device(q, {k_cache, v_cache, block_tables, seq_lens, query_start_loc, out},
-                     {status});
+                     {status, workspace});
   require_int4_attention(q, k_cache, v_cache, out, block_tables, seq_lens, status);
   TORCH_CHECK_TYPE(query_start_loc.scalar_type() == at::kInt, "query_start_loc must be int32");
   TORCH_CHECK_VALUE(query_start_loc.dim() == 1 &&
@@ -453,17 +454,26 @@ void require_int4_prefill(const at::Tensor& q, const at::Tensor& k_cache,
                         block_tables.size(0) >= num_seqs && seq_lens.numel() >= num_seqs,
                     "query_start_loc / block_tables / seq_lens too short for num_seqs");
   TORCH_CHECK_VALUE(max_q_len >= 0 && max_q_len <= INT32_MAX, "max_q_len out of range");
+  TORCH_CHECK_VALUE(!workspace.has_value() || workspace->is_contiguous(),
+                    "workspace must be contiguous");
 }
 
 void paged_prefill_int4(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
                         const at::Tensor& block_tables, const at::Tensor& seq_lens,
                         const at::Tensor& query_start_loc, at::Tensor& out, int64_t max_q_len,
                         double softmax_scale, int64_t num_seqs,
-                        const std::optional<at::Tensor>& status) {
+                        const std::optional<at::Tensor>& status,
+                        const std::optional<at::Tensor>& workspace) {
   require_int4_prefill(q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, out,
-                       max_q_len, num_seqs, status);
+                       max_q_len, num_seqs, status, workspace);
   const b200_int4_cache cache = int4_cache_desc(k_cache, v_cache);
   const c10::cuda::CUDAGuard guard(q.device());
+  // the caller's workspace, or one of this call on its stream
+  at::Tensor ws;
+  if (workspace.has_value())
+    ws = *workspace;
+  else if (num_seqs > 0 && q.size(0) > 0)
+    ws = at::empty({b200_paged_prefill_int4_workspace_bytes()}, q.options().dtype(at::kByte));
   check_int4(b200_paged_prefill_int4(q.data_ptr(), q.stride(0), q.stride(1),
                                      activation_dtype(q.scalar_type()), &cache,
                                      block_tables.data_ptr<int32_t>(), block_tables.stride(0),
@@ -475,8 +485,10 @@ void paged_prefill_int4(const at::Tensor& q, const at::Tensor& k_cache, const at
                                      static_cast<int32_t>(max_q_len),
                                      static_cast<int32_t>(q.size(1)), out.data_ptr(),
                                      out.stride(0), out.stride(1),
-                                     static_cast<float>(softmax_scale), status_ptr(status),
-                                     current_stream(q)),
+                                     static_cast<float>(softmax_scale),
+                                     ws.defined() ? ws.data_ptr() : nullptr,
+                                     ws.defined() ? ws.numel() * ws.element_size() : 0,
+                                     status_ptr(status), current_stream(q)),
              "paged_prefill");
 }
 
@@ -507,9 +519,10 @@ void paged_prefill_int4_meta(const at::Tensor& q, const at::Tensor& k_cache,
                              const at::Tensor& v_cache, const at::Tensor& block_tables,
                              const at::Tensor& seq_lens, const at::Tensor& query_start_loc,
                              at::Tensor& out, int64_t max_q_len, double, int64_t num_seqs,
-                             const std::optional<at::Tensor>& status) {
+                             const std::optional<at::Tensor>& status,
+                             const std::optional<at::Tensor>& workspace) {
   require_int4_prefill(q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, out,
-                       max_q_len, num_seqs, status);
+                       max_q_len, num_seqs, status, workspace);
 }
 
 // ------------------------------------------------ Meta (FakeTensor) kernels --
@@ -559,7 +572,8 @@ TORCH_LIBRARY(b200, m) {
   m.def(
       "paged_prefill_int4(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, "
       "Tensor seq_lens, Tensor query_start_loc, Tensor(a!) out, int max_q_len, "
-      "float softmax_scale, int num_seqs, Tensor(b!)? status=None) -> ()");
+      "float softmax_scale, int num_seqs, Tensor(b!)? status=None, "
+      "Tensor(c!)? workspace=None) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(b200, CUDA, m) {

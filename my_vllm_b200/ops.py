@@ -617,13 +617,15 @@ def paged_prefill(
     zeroed before its first use and again after a launch that reported an
     error) lets units much longer than the batch's average work per SM be
     split over several CTAs; launches sharing a workspace must not overlap.
-    Prefill over a 4-bit cache (``torch.uint8``) uses none."""
+    Over a 4-bit cache (``torch.uint8``) the workspace is one of
+    ``prefill_workspace_bytes(kv_int4=True)``, whose contents do not matter;
+    without one the call takes it from the caching allocator."""
     if k_cache.dtype == INT4_DTYPE and q.dtype != INT4_DTYPE:
         if k_scale is not None or v_scale is not None:
             raise ValueError("k_scale / v_scale apply to FP8 caches only")
         _int4_ops()[3](q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, out,
                        max_q_len, softmax_scale,
-                       seq_lens.numel() if num_seqs is None else num_seqs, status)
+                       seq_lens.numel() if num_seqs is None else num_seqs, status, workspace)
         return out
     for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache),
                     ("block_tables", block_tables), ("seq_lens", seq_lens),
@@ -651,7 +653,10 @@ def paged_prefill(
     return out
 
 
-@functools.lru_cache(maxsize=1)
-def prefill_workspace_bytes() -> int:
+@functools.lru_cache(maxsize=2)
+def prefill_workspace_bytes(*, kv_int4: bool = False) -> int:
     """Bytes of the optional prefill workspace (split-KV partial results)."""
-    return int(_native.load_library().b200_paged_prefill_workspace_bytes())
+    lib = _native.load_library()
+    if kv_int4:
+        return int(lib.b200_paged_prefill_int4_workspace_bytes())
+    return int(lib.b200_paged_prefill_workspace_bytes())

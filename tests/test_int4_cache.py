@@ -235,7 +235,7 @@ def test_c_abi_refuses_bad_caches(change, code, text):
                                            None),
         lambda: lib.b200_paged_prefill_int4(0x3000, 1024, 128, BF16, bad, 0x4000, 8, 8, 0x5000,
                                             0x7000, 4, 8, 2, 8, 0x6000, 1024, 128, 0.1, None,
-                                            None),
+                                            0, None, None),
     )
     for call in calls:
         assert call() == code
@@ -275,9 +275,10 @@ def test_c_abi_refuses_bad_rows_and_sizes():
     assert decode(ws=0x8010) == _native.B200_ERR_INVALID_ARGUMENT
     assert decode(n=0, q=None) == _native.B200_OK
 
-    def prefill(hq=8, q=0x3000, rows=8, most=2, scale=0.1, n=4):
+    def prefill(hq=8, q=0x3000, rows=8, most=2, scale=0.1, n=4, ws=None, nbytes=0):
         return lib.b200_paged_prefill_int4(q, 1024, 128, BF16, c, 0x4000, 8, 8, 0x5000, 0x7000, n,
-                                           rows, most, hq, 0x6000, 1024, 128, scale, None, None)
+                                           rows, most, hq, 0x6000, 1024, 128, scale, ws, nbytes,
+                                           None, None)
 
     assert prefill(hq=9) == _native.B200_ERR_INVALID_ARGUMENT
     assert prefill(hq=2 * 129) == _native.B200_ERR_UNSUPPORTED
@@ -286,4 +287,7 @@ def test_c_abi_refuses_bad_rows_and_sizes():
     assert prefill(scale=0.0) == _native.B200_ERR_INVALID_ARGUMENT
     assert prefill(scale=float("nan")) == _native.B200_ERR_INVALID_ARGUMENT
     assert prefill(rows=-1) == _native.B200_ERR_INVALID_ARGUMENT
+    assert prefill(ws=0x8010, nbytes=1 << 30) == _native.B200_ERR_INVALID_ARGUMENT
+    assert prefill(ws=0x8000, nbytes=4096) == _native.B200_ERR_INVALID_ARGUMENT
+    assert b"workspace" in lib.b200_last_error()
     assert prefill(rows=0, q=None) == _native.B200_OK

@@ -447,6 +447,91 @@ def test_prefill_rows_that_see_nothing(cuda_device, hq, hkv):
     assert (out[:50] == 0).all() and (out[50] != 0).any() and (out[190:] == 0).all()
 
 
+# (few units of many tiles, cut among SMs: parts, joins, cuts near a unit's ends)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("q,kv,hq,hkv", [([1], [5000], 4, 1), ([3, 70], [2100, 1500], 8, 2),
+                                         ([200], [3000], 5, 1), ([600], [4000], 2, 2)])
+def test_prefill_cut_units(cuda_device, dtype, q, kv, hq, hkv):
+    c = Case(q, kv, hq, hkv, 16, dtype, seed=len(kv))
+    out = _check_prefill(c, cuda_device)
+    assert torch.equal(out, _prefill(c, cuda_device))  # parts are joined in order
+
+
+def test_prefill_nan_in_one_part_of_a_cut_unit(cuda_device):
+    c = Case([40], [3000], 4, 1, 16, torch.bfloat16, seed=3)
+    ref, bounds = c.reference()
+    pages = int4.Pages(c.v.numpy())
+    for token, first in ((1000, 0), (2975, 15)):  # seen by every row, by rows 15 and up
+        page, row = divmod(c.slots[0][token], 16)
+        held = pages.scales[page, 0, row].copy()
+        pages.scales[page, 0, row].view(np.uint16)[2] = 0x7FC0
+        out = _prefill(c, cuda_device).cpu().double()
+        bad = torch.zeros(out.shape, dtype=torch.bool)
+        bad[first:, :, 64:96] = True
+        assert torch.equal(out.isnan(), bad)
+        assert_within(out.masked_fill(bad, 0.0), np.where(bad.numpy(), 0.0, ref),
+                      prefill_tolerance(ref, bounds, c.dtype))
+        pages.scales[page, 0, row] = held
+
+
+# (more than 128 blocks of rows, more units than a list of a CTA holds)
+@pytest.mark.parametrize("hq,hkv,n", [(8, 8, 330), (4, 1, 130), (20, 10, 250)])
+def test_prefill_many_sequences(cuda_device, hq, hkv, n):
+    q = [1 + (i % 3 == 0) - (i % 50 == 7) for i in range(n)]
+    kv = [max(q[i], (37 * i) % 150) for i in range(n)]
+    _check_prefill(Case(q, kv, hq, hkv, 16, torch.bfloat16, seed=n), cuda_device)
+
+
+def test_prefill_workspaces(cuda_device):
+    dev = cuda_device
+    c = Case([30], [2500], 4, 2, 16, torch.float16, seed=5)
+    want = _check_prefill(c, dev)
+    ws = torch.full((ops.prefill_workspace_bytes(kv_int4=True),), 255, dtype=torch.uint8, device=dev)
+    assert torch.equal(_prefill(c, dev, workspace=ws), want)
+    with pytest.raises(ValueError, match="workspace"):
+        _prefill(c, dev, workspace=ws[:4096])
+    with pytest.raises(ValueError, match="workspace"):
+        _prefill(c, dev, workspace=ws[8:])
+    with pytest.raises(ValueError, match="one device"):
+        _prefill(c, dev, workspace=ws.cpu())
+    # none at all, from C: whole units
+    q, k, v, tables, lens, starts = (x.to(dev) for x in (c.q, c.k, c.v, c.tables, c.lens, c.starts))
+    out = torch.full_like(q, float("nan"))
+    cache = _native.Int4Cache(k.data_ptr(), v.data_ptr(), k.size(0), 16, 2, k.stride(0))
+    rc = _native.load_library().b200_paged_prefill_int4(
+        q.data_ptr(), q.stride(0), q.stride(1), 0, cache, tables.data_ptr(), tables.stride(0),
+        tables.size(1), lens.data_ptr(), starts.data_ptr(), 1, 30, 30, 4, out.data_ptr(),
+        out.stride(0), out.stride(1), c.scale, None, 0, None,
+        torch.cuda.current_stream().cuda_stream)
+    assert rc == _native.B200_OK
+    ref, bounds = c.reference()
+    assert_within(out, ref, prefill_tolerance(ref, bounds, c.dtype))
+
+
+def test_prefill_graphs_share_a_workspace(cuda_device):
+    dev = cuda_device
+    ws = torch.empty(ops.prefill_workspace_bytes(kv_int4=True), dtype=torch.uint8, device=dev)
+    cases = [Case([30], [2500], 4, 2, 16, torch.bfloat16, seed=5),
+             Case([2, 3], [900, 1700], 4, 2, 32, torch.bfloat16, seed=6)]
+    wants = [_check_prefill(c, dev) for c in cases]
+    graphs = []
+    for c in cases:
+        q, k, v, tables, lens, starts = (x.to(dev) for x in (c.q, c.k, c.v, c.tables, c.lens,
+                                                             c.starts))
+        out = torch.empty_like(q)
+        args = (q, k, v, tables, lens, starts, out, max(c.q_lens), c.scale)
+        ops.paged_prefill(*args, workspace=ws)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.paged_prefill(*args, workspace=ws)
+        graphs.append((graph, out, args))
+    for _ in range(3):
+        for (graph, out, _args), want in zip(graphs, wants):
+            out.fill_(9.0)
+            graph.replay()
+            assert torch.equal(out, want)
+
+
 # ----------------------------------------------------------- used together --
 @pytest.mark.parametrize("dtype", TYPES)
 def test_a_prompt_then_steps_of_decoding(cuda_device, dtype):
