@@ -123,11 +123,13 @@ class B200PagedBackend(AttentionBackend):
     ) -> None:
         super().__init__(num_q_heads, num_kv_heads, head_dim, block_size, dtype)
         # Storage type of the paged caches: the activation dtype (the
-        # reference's only option) or FP8 E4M3 with per-layer scales attached
-        # through ops.register_kv_scales.
+        # reference's only option), FP8 E4M3 with per-layer scales attached
+        # through ops.register_kv_scales, or 4 bits (torch.uint8, pages of
+        # ops.int4_cache_shape) with scales of its own.
         self.kv_cache_dtype = dtype if kv_cache_dtype is None else kv_cache_dtype
-        if self.kv_cache_dtype not in (dtype, ops.FP8_DTYPE):
-            raise TypeError("kv_cache_dtype must be the backend dtype or torch.float8_e4m3fn")
+        if self.kv_cache_dtype not in (dtype, ops.FP8_DTYPE, ops.INT4_DTYPE):
+            raise TypeError("kv_cache_dtype must be the backend dtype, torch.float8_e4m3fn or "
+                            "torch.uint8 (4-bit)")
         reason = _static_support_reason(
             num_q_heads=num_q_heads, num_kv_heads=num_kv_heads, head_dim=head_dim,
             block_size=block_size, dtype=dtype,
@@ -219,6 +221,7 @@ class B200PagedBackend(AttentionBackend):
                 self.block_size, self._decode_max_kv_len(common), self.decode_num_parts,
                 total_kv_tokens=self._decode_total_kv_tokens(common),
                 kv_fp8=self.kv_cache_dtype == ops.FP8_DTYPE,
+                kv_int4=self.kv_cache_dtype == ops.INT4_DTYPE,
             )
         return B200PagedMetadata(
             common.query_start_loc, common.seq_lens, common.block_tables, decode_plan
@@ -283,7 +286,8 @@ class B200PagedBackend(AttentionBackend):
         ws = self._prefill_workspace
         if ws is None or ws.device != device:
             # zeroed once: every launch leaves its split counters at zero
-            ws = torch.zeros(ops.prefill_workspace_bytes(), dtype=torch.uint8, device=device)
+            nbytes = ops.prefill_workspace_bytes(kv_int4=self.kv_cache_dtype == ops.INT4_DTYPE)
+            ws = torch.zeros(nbytes, dtype=torch.uint8, device=device)
             self._prefill_workspace = ws
         return ws
 
@@ -437,7 +441,8 @@ class B200PagedBackend(AttentionBackend):
         decode_plan = ops.plan_decode(batch_size, self.num_q_heads, self.num_kv_heads,
                                       self.head_dim, self.block_size, max_kv_len,
                                       self.decode_num_parts,
-                                      kv_fp8=self.kv_cache_dtype == ops.FP8_DTYPE)
+                                      kv_fp8=self.kv_cache_dtype == ops.FP8_DTYPE,
+                                      kv_int4=self.kv_cache_dtype == ops.INT4_DTYPE)
         workspace = None
         if decode_plan.workspace_bytes:
             workspace = torch.empty(decode_plan.workspace_bytes, dtype=torch.uint8,
@@ -514,14 +519,16 @@ class B200PagedBackend(AttentionBackend):
             raise ValueError("query must be a CUDA tensor with the backend dtype")
         if q.ndim != 3 or q.shape[1:] != (self.num_q_heads, self.head_dim):
             raise ValueError("query must have shape [tokens, num_q_heads, head_dim]")
-        tail = (self.block_size, self.num_kv_heads, self.head_dim)
+        row = ops.INT4_ROW_BYTES if self.kv_cache_dtype == ops.INT4_DTYPE else self.head_dim
+        tail = (self.block_size, self.num_kv_heads, row)
         for name, cache in (("key", k_cache), ("value", v_cache)):
             if cache.device != q.device or cache.dtype != self.kv_cache_dtype:
                 raise ValueError(f"{name} cache must be on the query device with the "
                                  "backend's KV-cache dtype")
             if cache.ndim != 4 or cache.shape[1:] != tail:
                 raise ValueError(
-                    f"{name} cache must have shape [pages, block_size, num_kv_heads, head_dim]"
+                    f"{name} cache must have shape [pages, block_size, num_kv_heads, "
+                    f"{'head_dim' if row == self.head_dim else row}]"
                 )
 
 
