@@ -31,6 +31,18 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a B200 (sm_100a) GPU")
 
 
+def pytest_collection_modifyitems(items):
+    """Skips the single tests that take the backend, which is the engine's plugin,
+    in modules that do without it otherwise."""
+    if ENGINE_INSTALLED:
+        return
+    skip = pytest.mark.skip(reason="reference engine not installed in baseline/_ref")
+    for item in items:
+        code = getattr(getattr(item, "function", None), "__code__", None)
+        if code is not None and "B200PagedBackend" in code.co_names:
+            item.add_marker(skip)
+
+
 def pytest_report_header(config):
     if not ENGINE_INSTALLED:
         return "engine: nanovllm NOT installed in baseline/_ref (engine tests skip)"
