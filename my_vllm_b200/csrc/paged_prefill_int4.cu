@@ -12,24 +12,25 @@
 // scores, on the same four schedulers, which issue about one every other cycle.
 // So both are kept short, and their loops small: at 14 KB of hot code more than
 // a third of the fetches missed the instruction cache (1.8 ms for the first case
-// below instead of 1.1).
+// below, 1.3 once they were short).
 //
 // Work. A unit is (sequence, block of 256 packed rows, KV head): the (token, q
 // head of the group) rows of 256 / group query tokens, two UMMA M = 128 tiles A
 // and B that share every K and V tile of 128 tokens. Its cost is the tiles it
 // streams plus kUnitCost for its start and end. One CTA per SM; every CTA derives
 // its work from the lengths by itself, so the host needs none of them:
-//   * Shares below kSplitShare and no unit much above one: units whole, back and
-//     forth through the costliest-first order (at most 128 sequence blocks, ranked
-//     by each CTA).
+//   * Units all below a third of a share, or shares below kSplitShare and no unit
+//     much above one: units whole, back and forth through the costliest-first order
+//     (at most kOrder sequence blocks, ranked by each CTA).
 //   * Otherwise the sum of all costs is cut into equal shares, in unit order, one
 //     a CTA. A cut inside a unit leaves parts, whose sums (O, m, l in fp32) go to
 //     the workspace and are joined in part order by a second kernel; a cut within
 //     kMinPart tiles of a unit's end moves there. Without a workspace cuts move to
 //     the nearest end.
 // Measured (32 q heads, 8 KV heads, bf16; us): 2048 rows on 32k tokens, 256 equal
-// units on 148 SMs, whole 1370, cut 1100; 64 rows on 8k, 8 units, 191 and 44; four
-// chunks of 512 on 512 to 2560 tokens, 79 and 97; two prompts of 2048, 119 and 141.
+// units on 148 SMs, whole 1370, cut 1060 (1.01 PFLOP/s); 64 rows on 8k, 8 units,
+// 191 and 46; four chunks of 512 on 512 to 2560 tokens, 72 and 97; two prompts of
+// 2048, 111 and 141; one of 8192, 621 and 736.
 //
 // A CTA's 16 warps:
 //   0-3, 4-7  softmax of tile A, B: thread = row = TMEM lane. A row's 128 scores
@@ -83,6 +84,8 @@ constexpr int kV0 = kK0 + 2 * kTileBytes;
 constexpr int kOut0 = kV0 + 2 * kTileBytes;
 constexpr int kList0 = kOut0 + 8 * kOutBytes;
 
+constexpr int kOrder = 256;  // sequence blocks that are ranked: of 128 sequences at most
+
 // One unit, or part of one, of a CTA.
 struct Unit {
   int seq, kvh;
@@ -109,7 +112,7 @@ struct Shared {
   int2 scan_pairs[4];
   int seq, block, kvh;          // the next unit
   int whole;                    // units are dealt whole, from `order`
-  uint32_t order[128];          // (sequence << 16 | block) pairs, costliest first
+  uint16_t order[kOrder];       // (sequence << 9 | block) pairs, costliest first
   int count, tiles;             // of this round's list
   int dead;                     // a wait ran out
   uint32_t tmem;
@@ -117,7 +120,7 @@ struct Shared {
 constexpr int kSmemBytes = 1024 + kList0 + sizeof(Shared);
 static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 
-constexpr int kUnitCost = 2;  // of a unit besides its tiles, in tiles
+constexpr int kUnitCost = 3;  // of a unit besides its tiles, in tiles (2: 20000 rows 12 % slower)
 constexpr int kSplitShare = 64;  // shares from here on are always cut
 constexpr int kMinPart = 4;   // tiles of a part at least
 constexpr float kRescale = 8.f;  // log2
@@ -197,8 +200,9 @@ __device__ void find_share(const Int4PrefillParams& p, Shared* sh, int* scratch,
   }
   int64_t share = (total + gridDim.x - 1) / gridDim.x;
   if (share < kMinPart + kUnitCost - 1) share = kMinPart + kUnitCost - 1;
-  const bool whole = total_pairs <= 128 && p.num_seqs <= 65536 &&
-                     (p.records == nullptr || (share < kSplitShare && 4 * most <= 5 * share));
+  const bool whole =
+      total_pairs <= kOrder && p.num_seqs <= 128 &&
+      (p.records == nullptr || 3 * most <= share || (share < kSplitShare && 4 * most <= 5 * share));
   if (i == 0) sh->whole = whole;
   if (whole) {
     int id = first_pair;
@@ -207,15 +211,16 @@ __device__ void find_share(const Int4PrefillParams& p, Shared* sh, int* scratch,
       const int n = q.blocks(per);
       for (int b = 0; b < n; ++b, ++id) {
         scratch[id] = q.tiles(b, per) + kUnitCost;
-        scratch[128 + id] = (int)((uint32_t)s << 16 | b);
+        scratch[kOrder + id] = s << 9 | b;
       }
     }
     bar_sync(2, 128);
-    if (i < total_pairs) {
-      const int cost = scratch[i];
+    for (int at = i; at < total_pairs; at += 128) {
+      const int cost = scratch[at];
       int rank = 0;
-      for (int k = 0; k < total_pairs; ++k) rank += scratch[k] > cost || (scratch[k] == cost && k < i);
-      sh->order[rank] = scratch[128 + i];
+      for (int k = 0; k < total_pairs; ++k)
+        rank += scratch[k] > cost || (scratch[k] == cost && k < at);
+      sh->order[rank] = (uint16_t)scratch[kOrder + at];
     }
     if (i == 0) {
       sh->base = 0;
@@ -282,10 +287,10 @@ __device__ void list_units(const Int4PrefillParams& p, Shared* sh, bool first) {
     for (; n < kUnits; ++k) {
       const int64_t at = (int64_t)k * grid + (k & 1 ? grid - 1 - blockIdx.x : blockIdx.x);
       if (at >= units) break;
-      const uint32_t pair = sh->order[(int)at / p.cache.num_kv_heads];
-      const SeqInfo q = seq_info(p, pair >> 16);
-      const int b = pair & 0xffff, tiles = q.tiles(b, per);
-      put_unit(p, sh->units[n++], q, pair >> 16, b, (int)at % p.cache.num_kv_heads, 0, tiles, tiles);
+      const int pair = sh->order[(int)at / p.cache.num_kv_heads];
+      const SeqInfo q = seq_info(p, pair >> 9);
+      const int b = pair & 511, tiles = q.tiles(b, per);
+      put_unit(p, sh->units[n++], q, pair >> 9, b, (int)at % p.cache.num_kv_heads, 0, tiles, tiles);
       total += tiles;
     }
     sh->base = k;
@@ -720,9 +725,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // Warp m takes items m, m + 7, ..., 8 rows at a time: lane l holds the 32 codes
     // of group l / 8 of row l % 8, and writes 64 bytes of T as four chunks (no bank
-    // conflicts). Its codes and scales come straight from the cache: a row of
-    // registers is loaded for the next item as soon as this item's is converted,
-    // and that item's page ids one item earlier still.
+    // conflicts). Its codes and scales come straight from the cache: the registers
+    // are loaded for the next item as soon as this item is converted, and that
+    // item's page ids one item earlier still.
     const int c = lane >> 3;
     const uint32_t code_lane = (lane & 7) * kInt4CodeBytes + c * 16;
     const uint32_t scale_lane = p.cache.num_kv_heads * p.cache.block_size * kInt4CodeBytes +
@@ -794,7 +799,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           codes = base + (uint32_t)(x.row[r] * kInt4CodeBytes) + code_lane;
           scales = base + (uint32_t)(x.row[r] * kInt4ScaleBytes) + scale_lane;
         }
-        w[k] = *reinterpret_cast<const uint4*>(codes + (k & 1) * (8 * kInt4CodeBytes));
+        // read once by this SM: past L1, of which shared memory leaves little (4 % less
+        // time), and behind the conversions, not between them (1 %)
+        asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[k].x), "=r"(w[k].y), "=r"(w[k].z), "=r"(w[k].w)
+                     : "l"(codes + (k & 1) * (8 * kInt4CodeBytes)));
         bits[k] = *reinterpret_cast<const uint16_t*>(scales + (k & 1) * (8 * kInt4ScaleBytes));
       };
       Item now, next;
@@ -845,7 +854,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           auto row8 = [&](auto step) {
             constexpr int k = decltype(step)::value;
             convert32<k * 1024>(of(bits[k]), w[k], dst);
-            if (more) load(next, k);
           };
           row8(std::integral_constant<int, 0>());
           row8(std::integral_constant<int, 1>());
@@ -861,6 +869,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             rows([](uint32_t b) { return ConvertHalf<true>(b); });
           else
             rows([](uint32_t b) { return ConvertHalf<false>(b); });
+        }
+        if (more) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) load(next, k);
         }
         // generic writes of the tile -> the MMAs' async proxy
         fence_proxy_async_smem();

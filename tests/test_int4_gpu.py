@@ -482,6 +482,12 @@ def test_prefill_many_sequences(cuda_device, hq, hkv, n):
     _check_prefill(Case(q, kv, hq, hkv, 16, torch.bfloat16, seed=n), cuda_device)
 
 
+# (units much shorter than a CTA's share, dealt whole; more blocks than are ranked)
+@pytest.mark.parametrize("q,kv,hq,hkv", [([1100, 900], [1100, 1000], 64, 4), ([700], [700], 96, 1)])
+def test_prefill_many_blocks(cuda_device, q, kv, hq, hkv):
+    _check_prefill(Case(q, kv, hq, hkv, 16, torch.bfloat16, seed=hq), cuda_device)
+
+
 def test_prefill_workspaces(cuda_device):
     dev = cuda_device
     c = Case([30], [2500], 4, 2, 16, torch.float16, seed=5)
