@@ -959,7 +959,10 @@ int b200_paged_prefill_int4(const void* q, int64_t q_token_stride, int64_t q_hea
   p.div_mul = static_cast<uint32_t>((uint64_t(1) << (31 + s)) / c.block_size + 1);
   p.div_shift = s - 1;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  if (workspace) {
+  // tables that hold too few tokens for two parts: nothing to split, nothing to join
+  // (17 rows on 33 tokens: 14.5 us instead of 16.7)
+  const bool splits = (int64_t)max_blocks * c.block_size > 128 * (2 * b200::kInt4PrefillMinPart - 1);
+  if (workspace && splits) {
     p.joins = static_cast<int4*>(workspace);
     p.records = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
                                          b200::kInt4PrefillJoinBytes);

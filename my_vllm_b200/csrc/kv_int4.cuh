@@ -104,6 +104,7 @@ struct Int4PrefillParams {
   float* records;  // [2 num_ctas], or nullptr: no unit is split
   int32_t* status;
 };
+constexpr int kInt4PrefillMinPart = 4;  // 128-token tiles of a part of a split unit at least
 constexpr int kInt4PrefillCtas = 148;  // at most: one for each SM
 constexpr int64_t kInt4PrefillRecordBytes = 2 * 130 * 128 * 4;
 constexpr int64_t kInt4PrefillJoinBytes = (kInt4PrefillCtas * 16 + 255) / 256 * 256;

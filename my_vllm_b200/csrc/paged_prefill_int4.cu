@@ -113,7 +113,7 @@ struct Shared {
   int seq, block, kvh;          // the next unit
   int whole;                    // units are dealt whole, from `order`
   uint16_t order[kOrder];       // (sequence << 9 | block) pairs, costliest first
-  int count, tiles;             // of this round's list
+  int count, tiles;             // of the list
   int dead;                     // a wait ran out
   uint32_t tmem;
 };
@@ -121,8 +121,8 @@ constexpr int kSmemBytes = 1024 + kList0 + sizeof(Shared);
 static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 
 constexpr int kUnitCost = 3;  // of a unit besides its tiles, in tiles (2: 20000 rows 12 % slower)
+constexpr int kMinPart = kInt4PrefillMinPart;
 constexpr int kSplitShare = 64;  // shares from here on are always cut
-constexpr int kMinPart = 4;   // tiles of a part at least
 constexpr float kRescale = 8.f;  // log2
 
 __device__ __forceinline__ void bar_sync(int id, int threads) {
@@ -963,7 +963,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_sync(1, kThreads);
     }
     // every MMA issued has completed before TMEM is freed
-    if (lane == 0) {
+    if (elect_one()) {  // the lane that issued them
       umma_commit(smem_u32(&sh->drain));
       mbar_wait(smem_u32(&sh->drain), 0);
     }

@@ -457,6 +457,26 @@ def test_prefill_cut_units(cuda_device, dtype, q, kv, hq, hkv):
     assert torch.equal(out, _prefill(c, cuda_device))  # parts are joined in order
 
 
+@pytest.mark.parametrize("tokens", [896, 897, 1023, 1024, 1025])  # 7, 8 and 9 tiles
+def test_prefill_shortest_cut_units(cuda_device, tokens):
+    _check_prefill(Case([2], [tokens], 4, 1, 16, torch.float16, seed=tokens), cuda_device)
+
+
+def test_prefill_on_two_streams(cuda_device):
+    dev = cuda_device
+    c = Case([30], [2500], 4, 2, 16, torch.bfloat16, seed=5)
+    want = _check_prefill(c, dev)
+    args = [x.to(dev) for x in (c.q, c.k, c.v, c.tables, c.lens, c.starts)]
+    outs = [torch.empty_like(args[0]) for _ in range(8)]
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        with torch.cuda.stream(streams[i & 1]):
+            ops.paged_prefill(*args, out, 30, c.scale)
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for out in outs)
+
+
 def test_prefill_nan_in_one_part_of_a_cut_unit(cuda_device):
     c = Case([40], [3000], 4, 1, 16, torch.bfloat16, seed=3)
     ref, bounds = c.reference()
@@ -514,9 +534,12 @@ def test_prefill_workspaces(cuda_device):
     assert_within(out, ref, prefill_tolerance(ref, bounds, c.dtype))
 
 
-def test_prefill_graphs_share_a_workspace(cuda_device):
+@pytest.mark.parametrize("shared", [True, False])
+def test_prefill_graphs(cuda_device, shared):
+    # with one workspace, and with one that each graph takes from its own pool
     dev = cuda_device
     ws = torch.empty(ops.prefill_workspace_bytes(kv_int4=True), dtype=torch.uint8, device=dev)
+    ws = ws if shared else None
     cases = [Case([30], [2500], 4, 2, 16, torch.bfloat16, seed=5),
              Case([2, 3], [900, 1700], 4, 2, 32, torch.bfloat16, seed=6)]
     wants = [_check_prefill(c, dev) for c in cases]
