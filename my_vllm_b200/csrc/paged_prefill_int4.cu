@@ -3,7 +3,7 @@
 //
 // Row (token, q head) i of a sequence at position x attends to tokens t <= x:
 //   o_i = sum_t p_it v_t / sum_t p_it,  p_it = exp2(c q_i . k_t - m_i)
-// with k_t, v_t = s (code - 8) rounded to T, the type of q, and c = scale log2(e).
+// with k_t, v_t = s (code - 8) and c = scale log2(e).
 //
 // Bound: the MMAs (4 x 128 operations per row and token) and, right behind
 // them, an exp2 per row and token; the cache is 3.6 times smaller than in 16
@@ -29,8 +29,8 @@
 //     the nearest end.
 // Measured (32 q heads, 8 KV heads, bf16; us): 2048 rows on 32k tokens, 256 equal
 // units on 148 SMs, whole 1370, cut 1060 (1.01 PFLOP/s); 64 rows on 8k, 8 units,
-// 191 and 46; four chunks of 512 on 512 to 2560 tokens, 72 and 97; two prompts of
-// 2048, 111 and 141; one of 8192, 621 and 736.
+// 191 and 46; four chunks of 512 on 512 to 2560 tokens, 76 and 97; two prompts of
+// 2048, 119 and 141; one of 8192, 622 and 736.
 //
 // A CTA's 16 warps:
 //   0-3, 4-7  softmax of tile A, B: thread = row = TMEM lane. A row's 128 scores
@@ -50,8 +50,13 @@
 // 0 4 1 5 2 6 3 7. Q is staged in the same order, and O is put back in order
 // when it leaves; both are rare next to the tiles.
 //
-// Roundings: k and v to T, the MMAs' type (exact for fp16, 2^-8 of the value at most for bf16: s (c - 8)
-// has up to 11 bits); p to T, as its operand, while l sums it unrounded.
+// Roundings. The MMAs run in fp16 for bf16 calls too: s (c - 8) has up to 11 bits
+// and is exact there, and p loses 3 bits less (against the 64-bit result 0.0017 of
+// the output's norm, all of it the output's own rounding, where bf16 operands gave
+// 0.0032). bf16 queries become fp16 exactly, each row times a power of two. A unit
+// in which a scale leaves fp16's range is run a second time, with bf16 operands,
+// before the CTA's next units; its first results are overwritten. p is rounded to
+// the operands' type while l sums it unrounded.
 #include <cuda_runtime.h>
 #include <math.h>
 
@@ -97,7 +102,7 @@ struct Unit {
   int lim[2];    // tiles that A, B need: [0, lim)
   int rec;       // record of a part, or -1: the whole unit
   int nan[4];    // first token whose value group g has no finite scale
-  int pad;
+  int wide;      // bf16: 0, 1 when a scale is found to leave fp16's range, 2 the second run
 };
 static_assert(sizeof(Unit) == 64, "16 ints");
 
@@ -269,9 +274,10 @@ __device__ void put_unit(const Int4PrefillParams& p, Unit& u, const SeqInfo& q, 
   const int rows = u.ntok * p.group;
   u.lim[0] = tiles_to(q.len, u.pos0 + (min(kRows, rows) - 1) / p.group);
   u.lim[1] = rows > kRows ? tiles : 0;
-  u.rec = t0 > 0 ? 2 * blockIdx.x : t1 < tiles ? 2 * blockIdx.x + 1 : -1;
+  u.rec = t0 > 0 ? 2 * (int)blockIdx.x : t1 < tiles ? 2 * (int)blockIdx.x + 1 : -1;
 #pragma unroll
   for (int g = 0; g < 4; ++g) u.nan[g] = 0x7fffffff;
+  u.wide = 0;
 }
 
 // The next units of this CTA's share, by one thread.
@@ -337,6 +343,24 @@ __device__ void list_units(const Int4PrefillParams& p, Shared* sh, bool first) {
   sh->kvh = h;
   sh->count = n;
   sh->tiles = total;
+}
+
+// The units of the list that have to run again, in bf16; true if there are any.
+__device__ bool list_wide(Shared* sh) {
+  int n = 0, total = 0;
+  for (int e = 0; e < sh->count; ++e) {
+    if (sh->units[e].wide != 1) continue;
+    Unit& u = sh->units[n++];
+    u = sh->units[e];
+    u.wide = 2;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) u.nan[g] = 0x7fffffff;
+    total += u.t1 - u.t0;
+  }
+  if (n == 0) return false;
+  sh->count = n;
+  sh->tiles = total;
+  return true;
 }
 
 // A walk over the tiles of the list.
@@ -410,6 +434,12 @@ struct ConvertHalf {
   }
 };
 
+// Scales that bf16 calls do not multiply in fp16: from 2^13 (7 s overflows), and below
+// 2^-16, where a rounding of s and one of the product pass 2^-9 of the value each.
+__device__ __forceinline__ bool out_of_range(uint32_t bits) {
+  return bits - 1u < 0x377fu || bits - 0x4600u < 0x7f80u - 0x4600u;
+}
+
 // One lane's 32 codes -> four 16-byte chunks at shared addresses dst[j] + kOff.
 template <int kOff, typename C>
 __device__ __forceinline__ void convert32(const C& f, const uint4& w, const uint32_t (&dst)[4]) {
@@ -467,6 +497,7 @@ __device__ __forceinline__ float* record(float* records, int rec, int x) {
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     int4_prefill_kernel(const Int4PrefillParams p) {
+  constexpr bool kHalf = Elem<T>::kDtype == B200_DTYPE_FLOAT16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -539,15 +570,39 @@ __global__ void __launch_bounds__(kThreads, 1)
                    on);
       }
     };
-    auto order_q = [&] {
+    // in the tiles' order of columns; bf16 rows as fp16, each times a power of two
+    // that puts its largest element into [2^14, 2^15), which the row's scale undoes
+    float scale = p.scale_log2;  // of this thread's row in the unit whose Q is ordered
+    auto order_q = [&](int e) {
       asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll 4
+      const bool wide = sh->units[e].wide == 2;
+      int shift = 0;
+#pragma unroll 2
       for (int i = 0; i < 32; i += 2) {
         uint4* ptr = reinterpret_cast<uint4*>(qtile + (qc >> 3) * kHalfBytes + swz128(qr + i, qc & 7));
-        const uint4 v = *ptr;
+        uint4 v = *ptr;
+        if (!kHalf && !wide) {
+          uint32_t most = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                                   __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+          most = max(most & 0xffffu, most >> 16);
+#pragma unroll
+          for (int d = 1; d < 16; d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+          // no more than 2^126; rows with an infinity or a NaN as they are
+          const int k = most >= 0x7f80u ? 0 : min(126, 127 + 14 - (int)(most >> 7));
+          const float f = __uint_as_float((uint32_t)(127 + k) << 23);
+          auto half = [&](uint32_t w) {
+            return Elem<__half>::pack(__uint_as_float(w << 16) * f,
+                                      __uint_as_float(w & 0xffff0000u) * f);
+          };
+          v = make_uint4(half(v.x), half(v.y), half(v.z), half(v.w));
+          const int of_row = __shfl_sync(0xffffffffu, k, (lane & 1) * 16);
+          if ((lane & 30) == i) shift = of_row;
+        }
         *ptr = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
                           __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
       }
+      // never 0: masked scores are -inf, and stay so
+      if (!kHalf) scale = fmaxf(ldexpf(p.scale_log2, -shift), 1.1754944e-38f);
       fence_proxy_async_smem();
       mbar_arrive(smem_u32(&sh->q_full[x]));
     };
@@ -563,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int first = next_unit(0);
       if (first < sh->count) {
         stage_q(first);
-        order_q();
+        order_q(first);
       }
       for (int e = 0; e < sh->count && ok; ++e) {
         const Unit& u = sh->units[e];
@@ -571,6 +626,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int qpos = tl < u.ntok ? u.pos0 + tl : -1;
         const int seen = min(qpos + 1, u.seq_len);  // tokens this row sees
         float m = -INFINITY, l = 0.f;
+        const float row_scale = scale;
+        const bool wide = u.wide == 2;
         for (int j = t0; j < end; ++j) {
           const bool got = mbar_wait(smem_u32(&sh->s_full[x]), done & 1);
           if (!__all_sync(0xffffffffu, got)) {
@@ -608,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 64; ++i)
             mk[i & 3] = max3(mk[i & 3], sv[i >> 5][(2 * i) & 63], sv[i >> 5][(2 * i + 1) & 63]);
-          const float m_tile = max3(fmaxf(mk[0], mk[1]), mk[2], mk[3]) * p.scale_log2;
+          const float m_tile = max3(fmaxf(mk[0], mk[1]), mk[2], mk[3]) * row_scale;
           float alpha = 1.f;
           if (m_tile > m + kRescale) {
             alpha = fast_exp2(m - m_tile);
@@ -625,19 +682,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           const float base = m == -INFINITY ? 0.f : -m;
-          const uint64_t scale2 = f2(p.scale_log2, p.scale_log2), base2 = f2(base, base);
+          const uint64_t scale2 = f2(row_scale, row_scale), base2 = f2(base, base);
           uint64_t sum2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
+            float* pc = sv[c >> 1] + (c & 1) * 32;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               float x0, x1;
-              const float* pair = sv[c >> 1] + (c & 1) * 32 + 2 * i;
-              f2_split(f2_fma(f2(pair[0], pair[1]), scale2, base2), x0, x1);
-              const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-              sum2[i & 1] = f2_add(sum2[i & 1], f2(p0, p1));
-              pk[i] = Elem<T>::pack(p0, p1);
+              f2_split(f2_fma(f2(pc[2 * i], pc[2 * i + 1]), scale2, base2), x0, x1);
+              pc[2 * i] = ex2_approx(x0);
+              pc[2 * i + 1] = ex2_approx(x1);
+              sum2[i & 1] = f2_add(sum2[i & 1], f2(pc[2 * i], pc[2 * i + 1]));
+            }
+            uint32_t pk[16];
+            if (!kHalf && wide) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pk[i] = Elem<__nv_bfloat16>::pack(pc[2 * i], pc[2 * i + 1]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pk[i] = Elem<__half>::pack(pc[2 * i], pc[2 * i + 1]);
             }
             tmem_st16(tS + c * 16, pk);
             if (c & 1) {
@@ -650,7 +714,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           f2_split(sum2[0], s0, s1);
           f2_split(sum2[1], s2, s3);
           l = l * alpha + ((s0 + s1) + (s2 + s3));
-          if (j + 1 == end && next_unit(e + 1) < sh->count) order_q();
+          if (j + 1 == end) {
+            const int n = next_unit(e + 1);
+            if (n < sh->count) order_q(n);
+          }
         }
         if (ok && end > t0) {
           const bool got = mbar_wait(smem_u32(&sh->o_done[x]), units & 1);
@@ -739,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int turn = warp - kConvWarp;  // items until this warp's next
     int tiles = 0;                // of all rounds
     for (bool fresh = true;; fresh = false) {
-      if (i0 == 0) list_units(p, sh, fresh);
+      if (i0 == 0 && (fresh || kHalf || !list_wide(sh))) list_units(p, sh, fresh);
       bar_sync(1, kThreads);
       if (sh->dead || sh->count == 0) break;
       bool ok = true;
@@ -860,15 +927,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           row8(std::integral_constant<int, 2>());
           row8(std::integral_constant<int, 3>());
         };
-        if constexpr (Elem<T>::kDtype == B200_DTYPE_BFLOAT16) {
-          rows([](uint32_t b) { return ConvertBf16(b); });
-        } else {
+        const bool wide = sh->units[now.e].wide == 2;
+        if constexpr (kHalf) {
           using Small = ConvertHalf<true>;
           if (__any_sync(0xffffffffu, Small::small(bits[0]) || Small::small(bits[1]) ||
                                           Small::small(bits[2]) || Small::small(bits[3])))
             rows([](uint32_t b) { return ConvertHalf<true>(b); });
           else
             rows([](uint32_t b) { return ConvertHalf<false>(b); });
+        } else if (wide) {
+          rows([](uint32_t b) { return ConvertBf16(b); });
+        } else {
+          if (out_of_range(bits[0]) || out_of_range(bits[1]) || out_of_range(bits[2]) ||
+              out_of_range(bits[3])) {
+            Unit& u = sh->units[now.e];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)  // not past the end, where slots may hold anything
+              if (out_of_range(bits[k]) && first_token(now) + (lane & 7) + 8 * k < u.seq_len)
+                u.wide = 1;
+          }
+          rows([](uint32_t b) { return ConvertHalf<false>(b); });
         }
         if (more) {
 #pragma unroll
@@ -887,9 +965,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------------------------------------------------------- MMAs --
-    constexpr bool kBf16 = Elem<T>::kDtype == B200_DTYPE_BFLOAT16;
-    const uint32_t idesc_s = f16_instr_desc(kRows, kTokens, kBf16, false);
-    const uint32_t idesc_pv = f16_instr_desc(kRows, kHeadDim, kBf16, true);
+    auto desc = [](const Unit& u, bool pv) {
+      const bool wide = !kHalf && u.wide == 2;
+      return pv ? f16_instr_desc(kRows, kHeadDim, wide, true)
+                : f16_instr_desc(kRows, kTokens, wide, false);
+    };
     int pv0 = 0, pv1 = 0, qn0 = 0, qn1 = 0;  // tiles and units issued per Q tile
     int tiles = 0;
     while (true) {
@@ -915,7 +995,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (n >= 0 && cur.t < sh->units[cur.e].lim[x]) {  // PV of tile g
               const Unit& u = sh->units[cur.e];
               const uint64_t vd = smem_desc(sbase + kV0 + (g & 1) * kTileBytes, kHalfBytes, 1024);
-              const uint32_t par = (x ? pv1 : pv0) & 1;
+              const uint32_t par = (x ? pv1 : pv0) & 1, idesc_pv = desc(u, true);
               ok = mbar_wait(smem_u32(&sh->p_lo[x]), par) &&
                    mbar_wait(smem_u32(&sh->v_full[g & 1]), (g >> 1) & 1);
               if (!ok) break;
@@ -942,6 +1022,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               ok = mbar_wait(smem_u32(&sh->k_full[(g + 1) & 1]), ((g + 1) >> 1) & 1);
               if (!ok) break;
+              const uint32_t idesc_s = desc(sh->units[nxt.e], false);
               const uint64_t qd = smem_desc(sbase + kQ0 + x * kTileBytes, 16, 1024);
               const uint64_t kd = smem_desc(sbase + kK0 + ((g + 1) & 1) * kTileBytes, 16, 1024);
 #pragma unroll

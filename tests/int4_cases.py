@@ -62,9 +62,10 @@ def decode_tolerance(ref, bounds, dtype):
 
 
 def prefill_tolerance(ref, bounds, dtype):
-    """Prefill multiplies 16-bit operands: bf16 keys and values round s (c - 8)
-    (2^-8 each, in float16 it is exact), weights round to ``dtype``; scores stay
-    in fp32 as in decode."""
+    """Prefill multiplies 16-bit operands: fp16 ones, exact but for the weights,
+    or, for a bf16 call in which a scale leaves fp16's range, bf16 ones: keys and
+    values round s (c - 8) then (2^-8 each) and weights to bf16. bf16 calls get the
+    wider of the two bounds. Scores stay in fp32 as in decode."""
     u = UNIT[dtype]
     x = u if dtype == torch.bfloat16 else 0.0
     score = x * bounds["keys"] + 2.0 ** -19 * bounds["terms"]

@@ -369,6 +369,43 @@ def test_prefill_ranges(cuda_device, dtype, spread, v_spread):
     _check_prefill(c, cuda_device)
 
 
+# bf16 scales that leave fp16's range: all of them, or one value or key of one head
+@pytest.mark.parametrize("spread,v_spread", [(1.0, 2.0 ** 60), (1.0, 2.0 ** -60), (2.0 ** -60, 1.0),
+                                             (2.0 ** 18, 1.0), (1.0, 1e-6), (1e-6, 1e-6)])
+def test_prefill_wide_ranges(cuda_device, spread, v_spread):
+    c = Case([60, 20, 1], [60, 300, 2000], 4, 1, 16, torch.bfloat16, seed=9, spread=spread,
+             v_spread=v_spread)
+    c.scale = c.scale / max(spread, 1.0)
+    _check_prefill(c, cuda_device)
+
+
+@pytest.mark.parametrize("wide", [2.0 ** -40, 2.0 ** 17])
+@pytest.mark.parametrize("q,kv,hq,hkv", [([70, 20, 9], [150, 20, 300], 8, 2), ([40], [3000], 4, 1),
+                                         ([1] * 200, [130] * 200, 8, 8)])
+def test_prefill_one_wide_group(cuda_device, wide, q, kv, hq, hkv):
+    c = Case(q, kv, hq, hkv, 16, torch.bfloat16, seed=4)
+    token = c.slots[0][kv[0] - q[0]]
+    pages = int4.Pages(c.v.numpy())
+    page, row = divmod(token, 16)
+    bits = pages.scales[page, hkv - 1, row].view(np.uint16)
+    bits[1] = int(np.float32(wide).view(np.uint32) >> 16)
+    # and behind the end of the sequence, where it does not matter
+    for cache in (c.k, c.v):
+        last, used = divmod(c.slots[0][-1], 16)
+        if used < 15:
+            int4.Pages(cache.numpy()).scales[last, 0, 15].view(np.uint16)[:] = 0x7000
+    _check_prefill(c, cuda_device)
+
+
+@pytest.mark.parametrize("exponent", [-100, -40, 20, 100])
+def test_prefill_query_magnitudes(cuda_device, exponent):
+    c = Case([40, 3], [60, 500], 8, 2, 16, torch.bfloat16, seed=2)
+    c.q = (c.q.float() * 2.0 ** exponent).bfloat16()
+    c.q[5] = 0
+    c.scale = c.scale * 2.0 ** -exponent
+    _check_prefill(c, cuda_device)
+
+
 @pytest.mark.parametrize("hq,hkv", [(8, 2), (5, 1)])
 def test_prefill_leaves_other_rows(cuda_device, hq, hkv):
     # a sequence without new tokens in the middle, rows behind the last sequence
