@@ -8,7 +8,7 @@
 // Bound: the MMAs (4 x 128 operations per row and token) and, right behind
 // them, an exp2 per row and token; the cache is 3.6 times smaller than in 16
 // bits and never bounds. What does is the instructions of turning codes into
-// operands: 4 to 5 per pair of values next to the softmax's 7 per pair of
+// operands: 3 to 4 per pair of values next to the softmax's 7 per pair of
 // scores, on the same four schedulers, which issue about one every other cycle.
 // So both are kept short, and their loops small: at 14 KB of hot code more than
 // a third of the fetches missed the instruction cache (1.8 ms for the first case
