@@ -16,9 +16,13 @@
 // digit): the scales are bf16 as they are, the four sums of q are split into
 // three bf16 digits. 8 sum w adds up the weights as they were rounded, by additions
 // of fp16 to fp32. Roundings to 16 bits: q (exact: each head is scaled to [2^14,
-// 2^15) by a power of two first) and the weights w (fp16, 2^-11). The weights'
-// range is kept in fp16 by a running power of two over the value scales, which
-// takes part in the softmax's running maximum.
+// 2^15) by a power of two first) and the weights w (fp16, 2^-11). The weights are
+// kept in fp16's range by a power of two of each (head, group), which follows the
+// largest w seen, so that neither another group's scales nor a token that the head
+// hardly sees cost it bits; the softmax's maximum follows the scores alone. (One
+// power of two for a warp, over the scales, lost a group whose scales lay 2^24 below
+// another's. The multiplications and the check cost 1 to 6 %: 128 to 8192 tokens of
+// 124 sequences 142.4 to 144.1 us, one head of 512 rows 77.8 to 82.4.)
 //
 // Work split: the batch's 32-token tiles, in the order (sequence, KV head, tile),
 // are dealt to the CTAs in equal consecutive shares, whatever the sequences'
@@ -87,12 +91,15 @@ constexpr int kMinTiles = 4;
 // (8 sequences of 1 to 512 tokens, 8 KV heads: 7.6 us, cut 10.1).
 constexpr int kWholeTiles = 16;
 
-// Weights may grow to 2^kMostLog2 before the running maximum is moved (and O
-// rescaled); the largest one is 2^kHeadroom when it is, so fp16's normal range
+// Weights of a (head, group) may grow past kMostWeight before their power of two is
+// lowered; the largest one is about 2^kHeadroom when it is, so fp16's normal range
 // reaches 2^-14 / 2^kHeadroom below it.
-constexpr float kHeadroom = 6.f;
-constexpr int kMostLog2 = 14;
-constexpr int kMinScaleExp = 36;  // value scales below 2^-91 are not followed
+constexpr int kHeadroom = 6;
+constexpr uint32_t kMostWeight = 0x78007800;  // 2^15 twice, in fp16
+constexpr int kMostLift = 126;                // of the power of two
+// The softmax's base moves before a lane's sum of a tile passes this (fp32 holds
+// them all, so it moves for the first tile and hardly ever again).
+constexpr float kMostSum = 1152921504606846976.f;  // 2^60
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -196,6 +203,10 @@ __device__ __forceinline__ uint32_t rest_codes(uint32_t bytes, uint32_t even) {
   uint32_t r;
   asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(bytes), "r"(even));
   return r;
+}
+// 2^n; 0 below the normal range.
+__device__ __forceinline__ float pow2(int n) {
+  return n < -126 ? 0.f : __uint_as_float(static_cast<uint32_t>(min(n, 127) + 127) << 23);
 }
 __device__ __forceinline__ float lo_scale(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_scale(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
@@ -507,22 +518,23 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
     }
     __syncthreads();  // the queries (and the merge area is free again)
 
-    float m_run[kBlocks], base[kBlocks], l_run[kBlocks];
+    float base[kBlocks], l_run[kBlocks];  // base: whole numbers, so that rescaling is exact
+    uint64_t lift[4];  // 2^e of each group, of the lane's heads (one head: twice the same)
 #pragma unroll
     for (int c = 0; c < kBlocks; ++c) {
-      m_run[c] = base[c] = kNegInf;
+      base[c] = kNegInf;
       l_run[c] = 0.f;
     }
-    float o[8][4], ws[kBlocks][4];
+    // ws: sums of the weights by column of the lane's pair, as o has them
+    float o[8][4], ws[2][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-#pragma unroll
-      for (int c = 0; c < kBlocks; ++c) ws[c][i] = 0.f;
+      lift[i] = f2(pow2(kMostLift), pow2(kMostLift));
+      ws[0][i] = ws[1][i] = 0.f;
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt) o[mt][i] = 0.f;
     }
-    uint32_t ref = (kMinScaleExp << 7) | 0x7f;  // bf16 bits: the value scales stay at or below
-    float most = -1.f;  // 2^kMostLog2 in the weights' unit; -1: the first tile sets the maximum
+    float most = -1.f;  // the first tile sets the base and the lifts
 
     const int first = seg.begin + (seg.end - seg.begin) * warp / kWarps;
     const int last = seg.begin + (seg.end - seg.begin) * (warp + 1) / kWarps;
@@ -593,30 +605,35 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
 
         // ---- value scales of this lane's tokens, masked past the end ----
         uint2 vs[2][2];
-        vs[0][0] = lds64<kVScales>(sa);
-        vs[0][1] = lds64<kVScales + 64>(sa);
-        vs[1][0] = lds64<kVScales + 128>(sa);
-        vs[1][1] = lds64<kVScales + 192>(sa);
-        // the four lanes of a token look at one each of its row's four tokens
-        uint2 look = lds64<kVScales>(sa + tq * 64);
-        if (valid < kTile) {
-          // rows past the end may be any bytes; their codes are finite whatever they
-          // are, so a weight of exactly 0 needs the scale cleared
+        auto load_scales = [&]() {
+          vs[0][0] = lds64<kVScales>(sa);
+          vs[0][1] = lds64<kVScales + 64>(sa);
+          vs[1][0] = lds64<kVScales + 128>(sa);
+          vs[1][1] = lds64<kVScales + 192>(sa);
+          if (valid < kTile) {
+            // rows past the end may be any bytes; their codes are finite whatever they
+            // are, so a weight of exactly 0 needs the scale cleared
 #pragma unroll
-          for (int st = 0; st < 2; ++st)
+            for (int st = 0; st < 2; ++st)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (st * 16 + i * 8 + gr >= valid) {
-                vs[st][i] = make_uint2(0, 0);
+              for (int i = 0; i < 2; ++i)
+                if (st * 16 + i * 8 + gr >= valid) {
+                  vs[st][i] = make_uint2(0, 0);
 #pragma unroll
-                for (int blk = 0; blk < kBlocks; ++blk) sc[blk][st][i] = kNegInf;
-              }
-          if (tq * 8 + gr >= valid) look = make_uint2(0, 0);
-        }
+                  for (int blk = 0; blk < kBlocks; ++blk) sc[blk][st][i] = kNegInf;
+                }
+          }
+        };
+        load_scales();
 
-        // ---- weights; the running maximum and the value exponent move rarely ----
-        float pr[kBlocks][2][2], sum[kBlocks];
+        // ---- weights: p in fp32, then p vs 2^e in fp16 ----
+        // wt[st][g]: tokens g and g + 8 of head tq (one block), or heads tq and 4 + tq
+        // of token g, then of token g + 8
+        float sum[kBlocks];
+        uint32_t wt[2][4][kBlocks];
+        uint32_t top;  // the larger halves of all, and kMostWeight
         auto weigh = [&]() {
+          float pr[kBlocks][2][2];
 #pragma unroll
           for (int blk = 0; blk < kBlocks; ++blk) {
 #pragma unroll
@@ -626,42 +643,101 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
                 pr[blk][st][i] = ex2_approx(fmaf(sc[blk][st][i], fac[blk], -base[blk]));
             sum[blk] = (pr[blk][0][0] + pr[blk][0][1]) + (pr[blk][1][0] + pr[blk][1][1]);
           }
+          top = kMostWeight;
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            const uint2 v0 = vs[st][0], v1 = vs[st][1];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const uint32_t s0 = g < 2 ? v0.x : v0.y, s1 = g < 2 ? v1.x : v1.y;
+              const float f0 = (g & 1) ? hi_scale(s0) : lo_scale(s0);
+              const float f1 = (g & 1) ? hi_scale(s1) : lo_scale(s1);
+              float a, b;
+              if constexpr (kBlocks == 1) {
+                f2_split(f2_mul(f2_mul(f2(pr[0][st][0], pr[0][st][1]), f2(f0, f1)), lift[g]), a, b);
+                wt[st][g][0] = Elem<__half>::pack(a, b);
+              } else {
+                f2_split(f2_mul(f2_mul(f2(pr[0][st][0], pr[kBlocks - 1][st][0]), f2(f0, f0)), lift[g]),
+                         a, b);
+                wt[st][g][0] = Elem<__half>::pack(a, b);
+                f2_split(f2_mul(f2_mul(f2(pr[0][st][1], pr[kBlocks - 1][st][1]), f2(f1, f1)), lift[g]),
+                         a, b);
+                wt[st][g][kBlocks - 1] = Elem<__half>::pack(a, b);
+              }
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int c = 0; c < kBlocks; ++c) top = __vimax3_u16x2(top, wt[0][g][c], wt[1][g][c]);
         };
         weigh();
-        const uint32_t vmax2 = __vmaxu2(look.x, look.y);
-        const uint32_t vmax = max(vmax2 & 0xffffu, vmax2 >> 16);
-        if (__any_sync(0xffffffffu, vmax > ref || !(sum[0] <= most) || !(sum[kBlocks - 1] <= most))) {
-          // a scale that is no number spoils its own group's sums only: it is not followed
-          uint32_t top = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t w = i < 2 ? look.x : look.y;
-            const uint32_t s = (i & 1) ? w >> 16 : w & 0xffffu;
-            if (s < 0x7f80u) top = max(top, s);
-          }
-          ref = max(ref, __reduce_max_sync(0xffffffffu, top) | 0x7fu);
-          const int lift = static_cast<int>(ref >> 7) - 126;
-          most = __uint_as_float(static_cast<uint32_t>(127 + kMostLog2 - lift) << 23);
-          float alpha[kBlocks];
+        if (__any_sync(0xffffffffu, top != kMostWeight || !(sum[0] <= most) ||
+                                        !(sum[kBlocks - 1] <= most))) {
+          load_scales();  // again: they are not kept for this
+          // the base follows the scores alone
+          int up[kBlocks];  // by how much
 #pragma unroll
           for (int c = 0; c < kBlocks; ++c) {
             float m = fmaxf(fmaxf(sc[c][0][0], sc[c][0][1]), fmaxf(sc[c][1][0], sc[c][1][1])) * fac[c];
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            m_run[c] = fmaxf(m_run[c], m);
-            const float next = (m_run[c] == kNegInf ? 0.f : m_run[c]) +
-                               (static_cast<float>(lift) - kHeadroom);
-            alpha[c] = fminf(fast_exp2(base[c] - next), 1.f);
+            float next = fmaxf(base[c], floorf(m));
+            if (next == kNegInf) next = 0.f;
+            up[c] = most < 0.f ? 0 : static_cast<int>(fminf(next - base[c], 512.f));
             base[c] = next;
-            l_run[c] *= alpha[c];
+            l_run[c] *= pow2(-up[c]);
+          }
+          most = kMostSum;
+          // each (head, group)'s power of two follows its largest p vs: one that stands
+          // far above the rest costs them their bits only where it is all that counts. A
+          // scale that is no number spoils its own group's sums and is not followed
+          uint32_t high[kBlocks][2];  // exponents of p vs: groups 2 w | 2 w + 1 << 16
 #pragma unroll
-            for (int g = 0; g < 4; ++g) ws[c][g] *= alpha[c];
+          for (int c = 0; c < kBlocks; ++c) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                // below 2, so that a product with a finite scale is finite
+                const float pr = ex2_approx(fmaf(sc[c][st][i], fac[c], -base[c]));
+                x[0] = fmaxf(x[0], pr * lo_scale(vs[st][i].x));
+                x[1] = fmaxf(x[1], pr * hi_scale(vs[st][i].x));
+                x[2] = fmaxf(x[2], pr * lo_scale(vs[st][i].y));
+                x[3] = fmaxf(x[3], pr * hi_scale(vs[st][i].y));
+              }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              uint32_t e = __float_as_uint(x[2 * w]) >> 23 | (__float_as_uint(x[2 * w + 1]) >> 23) << 16;
+              e = __vmaxu2(e, __shfl_xor_sync(0xffffffffu, e, 4));
+              e = __vmaxu2(e, __shfl_xor_sync(0xffffffffu, e, 8));
+              high[c][w] = __vmaxu2(e, __shfl_xor_sync(0xffffffffu, e, 16));
+            }
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int g = 0; g < 4; ++g) {
+            float held[2], factor[2];
+            f2_split(lift[g], held[0], held[1]);
 #pragma unroll
-            for (int mt = 0; mt < 8; ++mt) o[mt][i] *= alpha[(i & 1) % kBlocks];
+            for (int c = 0; c < kBlocks; ++c) {
+              const int x = static_cast<int>(high[c][g >> 1] >> (g & 1) * 16 & 0xffffu);
+              const int old = static_cast<int>(__float_as_uint(held[c]) >> 23);
+              // (each + 127.) A higher base alone leaves p vs 2^e as it was; p vs < 2^(x - 126)
+              int e = min(old + up[c], kMostLift + 127);
+              if (e + x > 15 + 126 + 127 && x < 255) e = kHeadroom + 126 + 127 - x;
+              held[c] = __uint_as_float(static_cast<uint32_t>(e) << 23);
+              factor[c] = pow2(e - old - up[c]);
+            }
+            lift[g] = kBlocks == 1 ? f2(held[0], held[0]) : f2(held[0], held[1]);
+            if (kBlocks == 1) factor[1] = factor[0];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              o[2 * g][i] *= factor[i & 1];
+              o[2 * g + 1][i] *= factor[i & 1];
+              if (i < 2) ws[i][g] *= factor[i];
+            }
           }
           weigh();
         }
@@ -678,29 +754,23 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
           for (int g = 0; g < 4; ++g) {
             const uint32_t w0 = vw[2 * g], w1 = vw[2 * g + 1];  // tokens 0-7 | 8-15
             const uint32_t v0 = high_bytes(w0), v1 = high_bytes(w1);
-            const uint32_t s0 = g < 2 ? vs[st][0].x : vs[st][0].y;
-            const uint32_t s1 = g < 2 ? vs[st][1].x : vs[st][1].y;
-            const float f0 = (g & 1) ? hi_scale(s0) : lo_scale(s0);
-            const float f1 = (g & 1) ? hi_scale(s1) : lo_scale(s1);
             uint32_t b0, b1;
             if constexpr (kBlocks == 1) {
               // tokens g and g + 8 of head tq as columns 2 tq and 2 tq + 1: the even
               // columns sum over the first 8 tokens, the odd ones over the others
-              const uint32_t pair = Elem<__half>::pack(pr[0][st][0] * f0, pr[0][st][1] * f1);
-              add_low(ws[0][g], pair);
-              add_high(ws[0][g], pair);
-              const uint32_t w = movmatrix_trans(pair);
+              add_low(ws[0][g], wt[st][g][0]);
+              add_high(ws[1][g], wt[st][g][0]);
+              const uint32_t w = movmatrix_trans(wt[st][g][0]);
               b0 = w & first_half;
               b1 = w & ~first_half;
             } else {
-              const uint32_t p0 = Elem<__half>::pack(pr[0][st][0] * f0, pr[kBlocks - 1][st][0] * f0);
-              const uint32_t p1 = Elem<__half>::pack(pr[0][st][1] * f1, pr[kBlocks - 1][st][1] * f1);
-              add_low(ws[0][g], p0);
-              add_low(ws[0][g], p1);
-              add_high(ws[kBlocks - 1][g], p0);
-              add_high(ws[kBlocks - 1][g], p1);
-              b0 = movmatrix_trans(p0);
-              b1 = movmatrix_trans(p1);
+#pragma unroll
+              for (int i = 0; i < kBlocks; ++i) {
+                add_low(ws[0][g], wt[st][g][i]);
+                add_high(ws[1][g], wt[st][g][i]);
+              }
+              b0 = movmatrix_trans(wt[st][g][0]);
+              b1 = movmatrix_trans(wt[st][g][kBlocks - 1]);
             }
             mma_f16(o[2 * g], even_codes(w0), low_bytes(w0), even_codes(w1), low_bytes(w1), b0, b1);
             mma_f16(o[2 * g + 1], even_codes(v0), v0, even_codes(v1), v1, b0, b1);
@@ -713,6 +783,23 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
       lost = lost_next;
     }
 
+    // ---- 8 sum w off the sums of codes, 136 of them off the sums of bytes ----
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float w = ws[c][g];
+        w += __shfl_xor_sync(0xffffffffu, w, 4);
+        w += __shfl_xor_sync(0xffffffffu, w, 8);
+        w += __shfl_xor_sync(0xffffffffu, w, 16);
+        constexpr float kUnit = 5.9604644775390625e-8f;  // 2^-24, of a code
+#pragma unroll
+        for (int mt = 2 * g; mt < 2 * g + 2; ++mt) {
+          o[mt][c] = fmaf(w, -8.f * kUnit, o[mt][c]);
+          o[mt][2 + c] = fmaf(w, -136.f * kUnit, o[mt][2 + c]);
+        }
+      }
+
     // ---- merge the warps ----
     float* ml = reinterpret_cast<float*>(smem + L::kMerge);  // [warp][base | sum]
     float* mo = ml + kWarps * 2 * kHeads;                                   // [warp][head][stride]
@@ -721,12 +808,6 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
       l_run[c] += __shfl_xor_sync(0xffffffffu, l_run[c], 4);
       l_run[c] += __shfl_xor_sync(0xffffffffu, l_run[c], 8);
       l_run[c] += __shfl_xor_sync(0xffffffffu, l_run[c], 16);
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        ws[c][g] += __shfl_xor_sync(0xffffffffu, ws[c][g], 4);
-        ws[c][g] += __shfl_xor_sync(0xffffffffu, ws[c][g], 8);
-        ws[c][g] += __shfl_xor_sync(0xffffffffu, ws[c][g], 16);
-      }
       const int head = c * 4 + tq;
       if (head < heads) {
         constexpr float kUnit = 16777216.f, kUnit16 = 1048576.f;
@@ -734,13 +815,18 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
         auto total = [&](const float (&x)[4], int i) {
           return kBlocks == 1 ? x[2 * i] + x[2 * i + 1] : x[2 * i + c];
         };
+        const float own = 1.f / l_run[c];  // the warp's own result, which stays in range
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const float z = 8.f * ws[c][g];
+          float mine, other;
+          f2_split(lift[g], mine, other);
+          // 2^-e; a power of two, so nothing is rounded
+          const float down = __uint_as_float(0x7f000000u - __float_as_uint(c ? other : mine));
+          const float f = kUnit * own, f16 = kUnit16 * own;
           const float x0 = total(o[2 * g], 0), x2 = total(o[2 * g + 1], 0);
           *reinterpret_cast<float4*>(row + g * 32) =
-              make_float4(x0 * kUnit - z, (total(o[2 * g], 1) - x0) * kUnit16 - z, x2 * kUnit - z,
-                          (total(o[2 * g + 1], 1) - x2) * kUnit16 - z);
+              make_float4(x0 * f * down, (total(o[2 * g], 1) - x0) * f16 * down, x2 * f * down,
+                          (total(o[2 * g + 1], 1) - x2) * f16 * down);
         }
         if (gr == 0) {
           ml[warp * 2 * kHeads + head] = base[c];
@@ -758,25 +844,28 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
     for (int idx = threadIdx.x; idx < heads * (kHeadDim / 4); idx += blockDim.x) {
       const int head = idx >> 5;
       const int d = (idx & 31) * 4;
-      float m = kNegInf;
+      float m = kNegInf, l = 0.f, f[kWarps];
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w * 2 * kHeads + head]);
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      float l = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float mw = ml[w * 2 * kHeads + head];
-        if (mw == kNegInf) continue;  // a warp without tiles
-        const float f = fast_exp2(mw - m);
-        const float4 v = *reinterpret_cast<const float4*>(&mo[(w * kHeads + head) * kMergeStride + d]);
-        acc.x += v.x * f;
-        acc.y += v.y * f;
-        acc.z += v.z * f;
-        acc.w += v.w * f;
-        l += ml[w * 2 * kHeads + kHeads + head] * f;
+        f[w] = mw == kNegInf ? 0.f  // a warp without tiles
+                             : ml[w * 2 * kHeads + kHeads + head] * fast_exp2(mw - m);
+        l += f[w];
       }
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       const float inv = 1.f / l;
-      acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (ml[w * 2 * kHeads + head] == kNegInf) continue;
+        const float fw = f[w] * inv;
+        const float4 v = *reinterpret_cast<const float4*>(&mo[(w * kHeads + head) * kMergeStride + d]);
+        acc.x += v.x * fw;
+        acc.y += v.y * fw;
+        acc.z += v.z * fw;
+        acc.w += v.w * fw;
+      }
       if (whole) {
         uint32_t* ob = reinterpret_cast<uint32_t*>(
             static_cast<T*>(p.out) + (int64_t)seg.b * p.out_seq_stride +
