@@ -156,3 +156,15 @@ def test_a_token_without_a_finite_scale_beside_large_ones(cuda_device):
     assert torch.equal(out.isnan(), bad)
     assert_within(out.masked_fill(bad, 0.0), np.nan_to_num(ref),
                   np.nan_to_num(decode_tolerance(ref, bounds, c.dtype)))
+
+
+@pytest.mark.parametrize("n,parts", [(2048, 1), (32768, 1), (32768, 0), (131072, 1)])
+def test_flat_softmax_over_long_sequences(cuda_device, n, parts):
+    """Against 64 bits by norm. The weights' roundings (2^-11 of each, of either sign) add up
+    like the values themselves, so they stay 2^-11 of the result; its own is another 2^-11.
+    What grows with the length would be a bias of the sums, of which 2^-10 is left."""
+    c = Case([1], [n], 4, 1, 16, torch.float16, seed=n, spread=0.01)
+    out = _decode(c, cuda_device, parts).cpu().double().numpy()
+    ref, _ = c.reference()
+    err = np.linalg.norm(out - ref, axis=-1) / np.linalg.norm(ref, axis=-1)
+    assert err.max() <= 2.0 ** -9
