@@ -429,12 +429,13 @@ B200_API int b200_paged_decode_int4_plan(int32_t num_seqs, int32_t num_q_heads,
  * b200_paged_decode over a 4-bit cache; q and out are `dtype`. max_blocks is
  * the number of valid columns of block_tables: a token past them, or a page id
  * outside the pool, counts as a row of zeros and sets
- * B200_STATUS_PAGE_OUT_OF_RANGE. A sequence of length 0 gives zeros. `plan` is
- * one of b200_paged_decode_int4_plan and the workspace its workspace_bytes of
- * device memory, 256-byte aligned, whose contents mean nothing between calls;
- * calls that share one must not overlap on the GPU. The kernel is a
- * programmatic dependent of the kernel before it on `stream`, as
- * b200_paged_decode is, but reads nothing before that kernel has completed.
+ * B200_STATUS_PAGE_OUT_OF_RANGE. softmax_scale must be positive. A sequence of
+ * length 0 gives zeros. `plan` is one of b200_paged_decode_int4_plan and the
+ * workspace its workspace_bytes of device memory, 256-byte aligned, whose
+ * contents mean nothing between calls; calls that share one must not overlap on
+ * the GPU. The kernel is a programmatic dependent of the kernel before it on
+ * `stream`, as b200_paged_decode is, but reads nothing before that kernel has
+ * completed.
  */
 B200_API int b200_paged_decode_int4(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
                                     int32_t dtype, const b200_int4_cache* cache,

@@ -841,6 +841,8 @@ int b200_paged_decode_int4(const void* q, int64_t q_seq_stride, int64_t q_head_s
   if (plan->num_parts < 1 ||
       (plan->part_tokens != b200::kInt4DecodeTile && plan->part_tokens != 0))
     return fail(B200_ERR_INVALID_ARGUMENT, "the decode plan is not one for a 4-bit cache");
+  if (!(softmax_scale > 0.f))
+    return fail(B200_ERR_INVALID_ARGUMENT, "softmax_scale must be positive");
   if (num_seqs == 0) return B200_OK;
   if (!q || !out || !block_tables || !seq_lens)
     return fail(B200_ERR_INVALID_ARGUMENT, "NULL tensor pointer");

@@ -451,7 +451,6 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
   uint4* queries = reinterpret_cast<uint4*>(smem + L::kQuery);
   const uint32_t query = smem_u32(queries + lane);
   const uint32_t first_half = (gr & 1) ? 0u : 0xffffffffu;
-  const float sign = p.scale_log2 < 0.f ? -1.f : 1.f;  // the factor itself stays positive
 
   while (true) {
     const int kvh = seg.unit / p.splits;
@@ -477,9 +476,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       // 2^(14 - floor(log2 amax)), and back with the codes' 2^24
       const int e = max(static_cast<int>(__float_as_uint(amax) >> 23), 14);
-      const float up = __uint_as_float(static_cast<uint32_t>(268 - e) << 23) * sign;
+      const float up = __uint_as_float(static_cast<uint32_t>(268 - e) << 23);
+      // never 0: masked scores are -inf, and stay so
       const float down =
-          __uint_as_float(static_cast<uint32_t>(e) << 23) * 1024.f * fabsf(p.scale_log2);
+          fmaxf(__uint_as_float(static_cast<uint32_t>(e) << 23) * 1024.f * p.scale_log2, 1e-45f);
 #pragma unroll
       for (int c = 0; c < kBlocks; ++c) fac[c] = __shfl_sync(0xffffffffu, down, tq * 8 + c * 4);
       float own[4];

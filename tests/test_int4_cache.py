@@ -291,3 +291,19 @@ def test_c_abi_refuses_bad_rows_and_sizes():
     assert prefill(ws=0x8000, nbytes=4096) == _native.B200_ERR_INVALID_ARGUMENT
     assert b"workspace" in lib.b200_last_error()
     assert prefill(rows=0, q=None) == _native.B200_OK
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, float("nan"), float("-inf")])
+def test_attention_refuses_a_scale_that_is_not_positive(scale):
+    lib, c, plan = _native.load_library(), _cache(), _native.DecodePlan(2, 32, 0)
+    calls = (
+        lambda: lib.b200_paged_decode_int4(0x3000, 1024, 128, BF16, c, 0x4000, 8, 8, 0x5000, 4, 8,
+                                           0x6000, 1024, 128, scale, plan, 0x8000, 1 << 20, None,
+                                           None),
+        lambda: lib.b200_paged_prefill_int4(0x3000, 1024, 128, BF16, c, 0x4000, 8, 8, 0x5000,
+                                            0x7000, 4, 8, 2, 8, 0x6000, 1024, 128, scale, None, 0,
+                                            None, None),
+    )
+    for call in calls:
+        assert call() == _native.B200_ERR_INVALID_ARGUMENT
+        assert b"softmax_scale" in lib.b200_last_error()

@@ -168,3 +168,12 @@ def test_flat_softmax_over_long_sequences(cuda_device, n, parts):
     ref, _ = c.reference()
     err = np.linalg.norm(out - ref, axis=-1) / np.linalg.norm(ref, axis=-1)
     assert err.max() <= 2.0 ** -9
+
+
+@pytest.mark.parametrize("scale", [1e-3, 1e-30, 1e-44])
+def test_small_softmax_scales(cuda_device, scale):
+    # scores that vanish: means of the values, over partial tiles too
+    c = Case([1] * 2, [40, 33], 8, 2, 16, torch.float16, seed=2)
+    c.q[0] *= 2.0 ** -10
+    c.scale = scale
+    _check(c, cuda_device)
