@@ -53,10 +53,18 @@
 // Roundings. The MMAs run in fp16 for bf16 calls too: s (c - 8) has up to 11 bits
 // and is exact there, and p loses 3 bits less (against the 64-bit result 0.0017 of
 // the output's norm, all of it the output's own rounding, where bf16 operands gave
-// 0.0032). bf16 queries become fp16 exactly, each row times a power of two. A unit
-// in which a scale leaves fp16's range is run a second time, with bf16 operands,
-// before the CTA's next units; its first results are overwritten. p is rounded to
-// the operands' type while l sums it unrounded.
+// 0.0032). bf16 queries become fp16 exactly, each row times a power of two. p is
+// rounded to the operands' type while l sums it unrounded.
+//
+// A unit with a scale that fp16 does not hold is run a second time, before the CTA's
+// next units; its first results are overwritten. Keys are then multiplied by a power
+// of two that brings the unit's largest scale to 2^13 at most, and stay exact but for
+// what lies 2^25 and more below it; weights and values are bf16 (2^-8 each). fp16
+// calls need it as well: the cache has no type, and a value that overflows is 0 times
+// infinity in every row that does not see it. A converter warp looks closer where a
+// scale lies outside the octaves that it has met in the unit, so this costs two votes
+// and 20 instructions an item (chunks of 512 on 0 to 2048 tokens: 75.6 us without the
+// fp16 calls' run, 76.2 with it).
 #include <cuda_runtime.h>
 #include <math.h>
 
@@ -80,7 +88,7 @@ static_assert(256 * kSoftmaxRegs + 256 * kOtherRegs <= kThreads * 128, "register
 
 constexpr int kHalfBytes = kRows * 128;      // [128 rows x 64 columns]
 constexpr int kTileBytes = 2 * kHalfBytes;
-constexpr int kUnits = 16;  // of a CTA's list; longer lists run in rounds
+constexpr int kUnits = 15;  // of a CTA's list (as there is room for); longer lists run in rounds
 constexpr int kOutBytes = 32 * 128;  // 32 rows x 64 columns of output on their way, a warp
 // shared memory: Q A, B | K x 2 | V x 2 | output x 8 | list | barriers
 constexpr int kQ0 = 0;
@@ -102,9 +110,9 @@ struct Unit {
   int lim[2];    // tiles that A, B need: [0, lim)
   int rec;       // record of a part, or -1: the whole unit
   int nan[4];    // first token whose value group g has no finite scale
-  int wide;      // bf16: 0, 1 when a scale is found to leave fp16's range, 2 the second run
+  int wide;      // 0, 1 when a scale is found that fp16 operands do not hold, 2 the second run
+  uint32_t k_top;         // largest key scale, bf16 bits
 };
-static_assert(sizeof(Unit) == 64, "16 ints");
 
 struct Shared {
   Unit units[kUnits];
@@ -275,9 +283,10 @@ __device__ void put_unit(const Int4PrefillParams& p, Unit& u, const SeqInfo& q, 
   u.lim[0] = tiles_to(q.len, u.pos0 + (min(kRows, rows) - 1) / p.group);
   u.lim[1] = rows > kRows ? tiles : 0;
   u.rec = t0 > 0 ? 2 * (int)blockIdx.x : t1 < tiles ? 2 * (int)blockIdx.x + 1 : -1;
+  u.wide = 0;
+  u.k_top = 0;
 #pragma unroll
   for (int g = 0; g < 4; ++g) u.nan[g] = 0x7fffffff;
-  u.wide = 0;
 }
 
 // The next units of this CTA's share, by one thread.
@@ -345,7 +354,7 @@ __device__ void list_units(const Int4PrefillParams& p, Shared* sh, bool first) {
   sh->tiles = total;
 }
 
-// The units of the list that have to run again, in bf16; true if there are any.
+// The units of the list that have to run again; true if there are any.
 __device__ bool list_wide(Shared* sh) {
   int n = 0, total = 0;
   for (int e = 0; e < sh->count; ++e) {
@@ -404,10 +413,8 @@ template <bool kSmall>
 struct ConvertHalf {
   uint32_t mul;
   uint32_t post = 0x3c003c00u;
-  __device__ __forceinline__ static bool small(uint32_t bits) { return bits - 1u < 0x387fu; }
-  __device__ __forceinline__ explicit ConvertHalf(uint32_t bits) {
-    float s = __uint_as_float(bits << 16);
-    if (kSmall && small(bits)) {
+  __device__ __forceinline__ explicit ConvertHalf(float s) {
+    if (kSmall && s < 6.103515625e-5f) {
       s *= 256.f;
       post = 0x1c001c00u;
     }
@@ -434,10 +441,26 @@ struct ConvertHalf {
   }
 };
 
-// Scales that bf16 calls do not multiply in fp16: from 2^13 (7 s overflows), and below
-// 2^-16, where a rounding of s and one of the product pass 2^-9 of the value each.
-__device__ __forceinline__ bool out_of_range(uint32_t bits) {
-  return bits - 1u < 0x377fu || bits - 0x4600u < 0x7f80u - 0x4600u;
+// Whether fp16 holds s (c - 8) for scales from `low` (bf16 bits less one) to `top`. bf16
+// calls: from 2^13 on 7 s overflows, and below 2^-16 a rounding of s and one of the
+// product pass 2^-9 of the value each. fp16 calls: rows appended in fp16 have 9344 at
+// most; small values are as exact as the output is.
+template <bool kHalf>
+__device__ __forceinline__ bool fp16_holds(uint32_t low, uint32_t top) {
+  return kHalf ? top <= 0x4612u : top < 0x4600u && low >= 0x377fu;
+}
+// The ends of a scale's octave (so that not each new extreme is one), within what fp16
+// holds; 0 is none.
+template <bool kHalf>
+__device__ __forceinline__ uint32_t octave_top(uint32_t bits) {
+  return bits == 0 ? 0u : kHalf && bits <= 0x4612u ? min(bits | 0x7fu, 0x4612u) : bits | 0x7fu;
+}
+__device__ __forceinline__ uint32_t octave_low(uint32_t less_one) {
+  return ((less_one + 1u) & ~0x7fu) - 1u;
+}
+// What key scales are multiplied with in a second run, from the largest: to below 2^13.
+__device__ __forceinline__ int key_shift(uint32_t k_top) {
+  return k_top == 0 ? 0 : 139 - static_cast<int>(k_top >> 7);
 }
 
 // One lane's 32 codes -> four 16-byte chunks at shared addresses dst[j] + kOff.
@@ -581,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < 32; i += 2) {
         uint4* ptr = reinterpret_cast<uint4*>(qtile + (qc >> 3) * kHalfBytes + swz128(qr + i, qc & 7));
         uint4 v = *ptr;
-        if (!kHalf && !wide) {
+        if (!kHalf) {
           uint32_t most = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
                                    __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
           most = max(most & 0xffffu, most >> 16);
@@ -601,8 +624,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         *ptr = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
                           __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
       }
+      if (wide) shift += key_shift(sh->units[e].k_top);
       // never 0: masked scores are -inf, and stay so
-      if (!kHalf) scale = fmaxf(ldexpf(p.scale_log2, -shift), 1.1754944e-38f);
+      scale = fmaxf(ldexpf(p.scale_log2, -shift), 1.1754944e-38f);
       fence_proxy_async_smem();
       mbar_arrive(smem_u32(&sh->q_full[x]));
     };
@@ -696,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               sum2[i & 1] = f2_add(sum2[i & 1], f2(pc[2 * i], pc[2 * i + 1]));
             }
             uint32_t pk[16];
-            if (!kHalf && wide) {
+            if (wide) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) pk[i] = Elem<__nv_bfloat16>::pack(pc[2 * i], pc[2 * i + 1]);
             } else {
@@ -806,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int turn = warp - kConvWarp;  // items until this warp's next
     int tiles = 0;                // of all rounds
     for (bool fresh = true;; fresh = false) {
-      if (i0 == 0 && (fresh || kHalf || !list_wide(sh))) list_units(p, sh, fresh);
+      if (i0 == 0 && (fresh || !list_wide(sh))) list_units(p, sh, fresh);
       bar_sync(1, kThreads);
       if (sh->dead || sh->count == 0) break;
       bool ok = true;
@@ -855,6 +879,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t bits[4];
       const uint8_t *codes, *scales;
       int bad = 0;  // runs of the loaded item outside the table or the pool
+      // bits of the scales met so far in unit `met`, of keys and of this lane's value group:
+      // the largest, and the smallest but 0 less one; whether any is below 2^-14
+      int met = -1;
+      uint32_t k_top = 0, k_low = 0, v_top = 0, v_low = 0;
+      bool k_small = false, v_small = false;
       // rows 8 k + l % 8 of the item, k = 2 r and 2 r + 1: run r
       auto load = [&](const Item& x, int k) {
         if ((k & 1) == 0) {
@@ -897,11 +926,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (bad & 1) bits[0] = bits[1] = 0;
           if (bad & 2) bits[2] = bits[3] = 0;
         }
+        const bool more = next.e >= 0;
+        Unit& u = sh->units[now.e];
+        const bool wide = u.wide == 2;
+        if (met != now.e) {
+          met = now.e;
+          k_top = v_top = 0;
+          k_low = v_low = 0xffffffffu;
+          k_small = v_small = false;
+        }
+        const int tok0 = first_token(now) + (lane & 7);
+        auto ends = [&](uint32_t& top, uint32_t& low) {
+          top = max(max(bits[0], bits[1]), max(bits[2], bits[3]));
+          low = min(min(bits[0] - 1u, bits[1] - 1u), min(bits[2] - 1u, bits[3] - 1u));
+        };
+        uint32_t top, low;
+        ends(top, low);
         if (now.is_v) {
-          Unit& u = sh->units[now.e];
-          const int tok0 = first_token(now) + (lane & 7);
-          const uint32_t top = max(max(bits[0], bits[1]), max(bits[2], bits[3]));
-          if (__any_sync(0xffffffffu, top >= 0x7f80u || tok0 + 24 >= u.seq_len)) {
+          if (__any_sync(0xffffffffu, top > v_top || low < v_low || tok0 + 24 >= u.seq_len)) {
             // a row past the end counts as zeros (its slot may hold anything), and so
             // does a group without a finite scale, whose token is remembered: rows
             // that see it get NaN when O leaves, rows before it do not
@@ -914,9 +956,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                 bits[k] = 0;
               }
             }
+            ends(top, low);
+            v_top = max(v_top, octave_top<kHalf>(top));
+            v_low = min(v_low, octave_low(low));
+            v_small = __any_sync(0xffffffffu, v_low < 0x387fu);
+            if (!wide && !fp16_holds<kHalf>(v_low, v_top)) u.wide = 1;
+          }
+        } else if (__any_sync(0xffffffffu, top > k_top || low < k_low)) {
+          // past the end slots hold anything, and a scale that is no number spoils its
+          // rows in any type
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (tok0 + 8 * k < u.seq_len && bits[k] < 0x7f80u) {
+              k_top = max(k_top, octave_top<kHalf>(bits[k]));
+              k_low = min(k_low, octave_low(bits[k] - 1u));
+            }
+          // of all groups and rows: the smallest keys only count if all are small
+          k_top = __reduce_max_sync(0xffffffffu, k_top);
+          k_low = __reduce_min_sync(0xffffffffu, k_low);
+          k_small = k_low < 0x387fu;
+          if (!wide) {
+            k_top = max(k_top, atomicMax(&u.k_top, k_top));
+            if (!fp16_holds<kHalf>(k_low, k_top) ||
+                (kHalf && k_top < 0x3b00u && k_low < 0x36ffu))  // 2^-9, 2^-17
+              u.wide = 1;
           }
         }
-        const bool more = next.e >= 0;
         auto rows = [&](auto of) {
           auto row8 = [&](auto step) {
             constexpr int k = decltype(step)::value;
@@ -927,26 +992,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           row8(std::integral_constant<int, 2>());
           row8(std::integral_constant<int, 3>());
         };
-        const bool wide = sh->units[now.e].wide == 2;
-        if constexpr (kHalf) {
-          using Small = ConvertHalf<true>;
-          if (__any_sync(0xffffffffu, Small::small(bits[0]) || Small::small(bits[1]) ||
-                                          Small::small(bits[2]) || Small::small(bits[3])))
-            rows([](uint32_t b) { return ConvertHalf<true>(b); });
-          else
-            rows([](uint32_t b) { return ConvertHalf<false>(b); });
-        } else if (wide) {
-          rows([](uint32_t b) { return ConvertBf16(b); });
-        } else {
-          if (out_of_range(bits[0]) || out_of_range(bits[1]) || out_of_range(bits[2]) ||
-              out_of_range(bits[3])) {
-            Unit& u = sh->units[now.e];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)  // not past the end, where slots may hold anything
-              if (out_of_range(bits[k]) && first_token(now) + (lane & 7) + 8 * k < u.seq_len)
-                u.wide = 1;
+        if (wide) {
+          if (now.is_v) {
+            rows([](uint32_t b) { return ConvertBf16(b); });
+          } else {
+            const int shift = key_shift(u.k_top);
+            const float f0 = ldexpf(1.f, shift / 2), f1 = ldexpf(1.f, shift - shift / 2);
+            rows([&](uint32_t b) { return ConvertHalf<true>(__uint_as_float(b << 16) * f0 * f1); });
           }
-          rows([](uint32_t b) { return ConvertHalf<false>(b); });
+        } else if (kHalf && (now.is_v ? v_small : k_small)) {
+          rows([](uint32_t b) { return ConvertHalf<true>(__uint_as_float(b << 16)); });
+        } else {
+          rows([](uint32_t b) { return ConvertHalf<false>(__uint_as_float(b << 16)); });
         }
         if (more) {
 #pragma unroll
@@ -965,11 +1022,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------------------------------------------------------- MMAs --
-    auto desc = [](const Unit& u, bool pv) {
-      const bool wide = !kHalf && u.wide == 2;
-      return pv ? f16_instr_desc(kRows, kHeadDim, wide, true)
-                : f16_instr_desc(kRows, kTokens, wide, false);
-    };
+    // S in fp16; PV in bf16 in a second run
+    const uint32_t idesc_s = f16_instr_desc(kRows, kTokens, false, false);
     int pv0 = 0, pv1 = 0, qn0 = 0, qn1 = 0;  // tiles and units issued per Q tile
     int tiles = 0;
     while (true) {
@@ -995,7 +1049,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (n >= 0 && cur.t < sh->units[cur.e].lim[x]) {  // PV of tile g
               const Unit& u = sh->units[cur.e];
               const uint64_t vd = smem_desc(sbase + kV0 + (g & 1) * kTileBytes, kHalfBytes, 1024);
-              const uint32_t par = (x ? pv1 : pv0) & 1, idesc_pv = desc(u, true);
+              const uint32_t par = (x ? pv1 : pv0) & 1;
+              const uint32_t idesc_pv = f16_instr_desc(kRows, kHeadDim, u.wide == 2, true);
               ok = mbar_wait(smem_u32(&sh->p_lo[x]), par) &&
                    mbar_wait(smem_u32(&sh->v_full[g & 1]), (g >> 1) & 1);
               if (!ok) break;
@@ -1022,7 +1077,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               ok = mbar_wait(smem_u32(&sh->k_full[(g + 1) & 1]), ((g + 1) >> 1) & 1);
               if (!ok) break;
-              const uint32_t idesc_s = desc(sh->units[nxt.e], false);
               const uint64_t qd = smem_desc(sbase + kQ0 + x * kTileBytes, 16, 1024);
               const uint64_t kd = smem_desc(sbase + kK0 + ((g + 1) & 1) * kTileBytes, 16, 1024);
 #pragma unroll

@@ -81,3 +81,35 @@ def assert_within(out, ref, tol):
         f"{(over > 0).sum()} of {over.size} values off, worst "
         f"{np.abs(got - ref).flat[over.argmax()]:.3e} where {tol.flat[over.argmax()]:.3e} is "
         f"allowed, at {np.unravel_index(over.argmax(), over.shape)}")
+
+
+def prefill_bound(ref, bounds, dtype, wide=False):
+    """The bound of prefill by the operands that a unit really runs with. fp16: keys and
+    values are exact and weights round by 2^-11 (those below 2^-21 of a row's largest
+    round to multiples of 2^-32 of it: that, for values whose scales lie up to 2^18
+    apart, is within the 2^-19 that covers the exponentials). ``wide``: weights and
+    values in bf16, keys still exact. Scores stay in fp32 as in decode. fp16 outputs
+    below its normal range are off by half their step, 2^-25."""
+    bf16 = UNIT[torch.bfloat16]
+    rounded = 2 * bf16 + bf16 ** 2 if wide else UNIT[torch.float16]
+    weight = rounded + 2.0 ** -19 + np.expm1(2 * 2.0 ** -19 * bounds["terms"])[..., None]
+    u = UNIT[dtype]
+    least = 2.0 ** -25 if dtype == torch.float16 else 1e-37
+    return u * np.abs(ref) + weight * bounds["mass"] * (1 + u) + least
+
+
+def assert_near(out, ref, dtype, wide=False, carried=128):
+    """By norm, over each output row [128]. A rounding to a unit of u is uniform within u of
+    the value's power of two, whose square is 0.5435 of the value's in the mean at most
+    (normal values of any deviation), so independent ones come to u sqrt(0.5435 / 3) of a
+    row: the output's own, and, wide, the values'. Their squares, 3.5 / n of them in
+    variance where n normal values carry the row, scatter by sqrt(3.5 / n), so the norm by
+    half of that; four of these are left. A token's weight has one rounding for all its
+    values: up to u by norm where one token carries the row, and 1.2 u where a few do that
+    are not orthogonal."""
+    own, operand = UNIT[dtype], UNIT[torch.bfloat16 if wide else torch.float16]
+    spread = (1 + 2 * np.sqrt(3.5 / carried)) ** 2 * 0.5435 / 3
+    limit = np.sqrt(spread * (own ** 2 + (operand ** 2 if wide else 0)) + (1.2 * operand) ** 2)
+    err = np.linalg.norm(out.detach().double().cpu().numpy() - ref, axis=-1)
+    ratio = err / np.maximum(np.linalg.norm(ref, axis=-1), 1e-37)
+    assert ratio.max() <= limit, f"a row is {ratio.max():.2e} off by norm, {limit:.2e} is allowed"
