@@ -7,7 +7,7 @@ import torch
 
 from conftest import dtype_name, storage
 from int4_cases import Case, assert_near, assert_within, prefill_bound
-from my_vllm_b200 import ops
+from my_vllm_b200 import _native, ops
 from oracle import int4
 
 pytestmark = pytest.mark.gpu
@@ -39,6 +39,34 @@ def _rewrite(c, key=None, value=None, dtype=None):
 
 def _groups(*exponents):
     return torch.repeat_interleave(2.0 ** torch.tensor(exponents, dtype=torch.float64), 32)
+
+
+# few units of many tiles (parts, joins), whole ones, ragged ones
+SHAPES = [([1], [5000], 4, 1), ([200], [3000], 5, 1), ([600], [4000], 2, 2), ([30], [2500], 4, 2),
+          ([60, 20, 1], [60, 300, 2000], 4, 1), ([300, 129], [300, 640], 8, 2)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("q,kv,hq,hkv", SHAPES)
+def test_long_contexts(cuda_device, dtype, q, kv, hq, hkv):
+    _check(Case(q, kv, hq, hkv, 16, dtype, seed=kv[0]), cuda_device)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("spread,v_spread", [(4.0, 1.0), (1.0, 0.02), (0.05, 50.0)])
+def test_scales_within_fp16(cuda_device, dtype, spread, v_spread):
+    c = Case([60, 20, 200], [60, 300, 1500], 8, 2, 32, dtype, seed=3, spread=spread,
+             v_spread=v_spread)
+    _check(c, cuda_device)
+
+
+@pytest.mark.parametrize("exponent", [-100, -30, 20, 100])
+def test_queries_of_any_magnitude(cuda_device, exponent):
+    c = Case([40, 3], [60, 2500], 8, 2, 16, torch.bfloat16, seed=2)
+    c.q = (c.q.float() * 2.0 ** exponent * torch.linspace(1, 2 ** 10, 43)[:, None, None]).bfloat16()
+    c.q[5] = 0
+    c.scale = c.scale * 2.0 ** -exponent / 2 ** 10
+    _check(c, cuda_device)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -93,3 +121,38 @@ def test_groups_far_apart(cuda_device, dtype, exponents):
     c = Case([60, 20], [60, 1200], 8, 2, 16, dtype, seed=6)
     _rewrite(c, value=c.value.double() * _groups(*exponents))
     _check(c, cuda_device, wide=max(exponents) > 12 or min(exponents) < -12, carried=32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("column", [1, 2, 5, 6])
+@pytest.mark.parametrize("bad", [-1, 1 << 30])
+def test_a_bad_page_counts_as_rows_of_zeros(cuda_device, dtype, column, bad):
+    q, kv = [20, 20], [130, 20]
+    c = Case(q, kv, 4, 2, 16, dtype, seed=1)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    keep = c.tables.clone()
+    c.tables[0, column] = bad
+    out = _prefill(c, cuda_device, status=status)
+    assert int(status) == _native.STATUS_PAGE_OUT_OF_RANGE
+    c.tables = keep
+    for slot in c.slots[0][16 * column: 16 * column + 16]:
+        for cache in (c.k, c.v):
+            int4.Pages(cache.numpy()).put(slot, np.full((2, 128), 8, np.uint8), np.zeros((2, 4)))
+    ref, bounds = c.reference()
+    assert_within(out, ref, prefill_bound(ref, bounds, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_tokens_past_the_table_count_as_rows_of_zeros(cuda_device, dtype):
+    c = Case([20, 20], [96, 20], 4, 2, 16, dtype, seed=1)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    q, k, v, lens, starts = (x.to(cuda_device) for x in (c.q, c.k, c.v, c.lens, c.starts))
+    short = c.tables[:, :5].contiguous().to(cuda_device)  # 80 of the 96 tokens
+    out = torch.full_like(q, float("nan"))
+    ops.paged_prefill(q, k, v, short, lens, starts, out, 20, c.scale, status=status)
+    assert int(status) == _native.STATUS_PAGE_OUT_OF_RANGE
+    for slot in c.slots[0][80:]:
+        for cache in (c.k, c.v):
+            int4.Pages(cache.numpy()).put(slot, np.full((2, 128), 8, np.uint8), np.zeros((2, 4)))
+    ref, bounds = c.reference()
+    assert_within(out, ref, prefill_bound(ref, bounds, dtype))
