@@ -112,6 +112,7 @@ struct Unit {
   int nan[4];    // first token whose value group g has no finite scale
   int wide;      // 0, 1 when a scale is found that fp16 operands do not hold, 2 the second run
   uint32_t k_top;         // largest key scale, bf16 bits
+  uint32_t v_octaves[4];  // of value group g's scales, the ends: bit i from 2^(i - 18) on, 0 also below
 };
 
 struct Shared {
@@ -137,6 +138,10 @@ constexpr int kUnitCost = 3;  // of a unit besides its tiles, in tiles (2: 20000
 constexpr int kMinPart = kInt4PrefillMinPart;
 constexpr int kSplitShare = 64;  // shares from here on are always cut
 constexpr float kRescale = 8.f;  // log2
+// fp16 weights are multiplied by 2^7 (2^15 at most, by kRescale): those down to 2^-21 of
+// a row's largest are normal numbers there. bf16 ones stay at or below 1, so that sums of
+// the largest values are finite.
+constexpr float kWeightLift = 7.f;
 
 __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
@@ -286,7 +291,10 @@ __device__ void put_unit(const Int4PrefillParams& p, Unit& u, const SeqInfo& q, 
   u.wide = 0;
   u.k_top = 0;
 #pragma unroll
-  for (int g = 0; g < 4; ++g) u.nan[g] = 0x7fffffff;
+  for (int g = 0; g < 4; ++g) {
+    u.nan[g] = 0x7fffffff;
+    u.v_octaves[g] = 0;
+  }
 }
 
 // The next units of this CTA's share, by one thread.
@@ -449,6 +457,12 @@ template <bool kHalf>
 __device__ __forceinline__ bool fp16_holds(uint32_t low, uint32_t top) {
   return kHalf ? top <= 0x4612u : top < 0x4600u && low >= 0x377fu;
 }
+// Weights below 2^-21 of a row's largest are multiples of 2^-32 of it, which is less
+// than the roundings of the others while the values of a group lie within 2^18.
+constexpr int kApart = 18;
+__device__ __forceinline__ uint32_t octave(uint32_t bits) {
+  return 1u << min(max(static_cast<int>(bits >> 7) - (127 - 18), 0), 31);
+}
 // The ends of a scale's octave (so that not each new extreme is one), within what fp16
 // holds; 0 is none.
 template <bool kHalf>
@@ -512,7 +526,7 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool o
                : "memory");
 }
 
-// A record: [130][128 rows] floats, 128 columns of O (in tile order), m and l.
+// A record: [130][128 rows] floats, 128 columns of O (in tile order), their base 2^m and l.
 __device__ __forceinline__ float* record(float* records, int rec, int x) {
   return records + ((int64_t)rec * 2 + x) * (130 * kRows);
 }
@@ -652,6 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float m = -INFINITY, l = 0.f;
         const float row_scale = scale;
         const bool wide = u.wide == 2;
+        const float weight_lift = wide ? -kRescale : kWeightLift;
         for (int j = t0; j < end; ++j) {
           const bool got = mbar_wait(smem_u32(&sh->s_full[x]), done & 1);
           if (!__all_sync(0xffffffffu, got)) {
@@ -705,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_st16(tO + c * 16, o);
             }
           }
-          const float base = m == -INFINITY ? 0.f : -m;
+          const float base = m == -INFINITY ? 0.f : weight_lift - m;
           const uint64_t scale2 = f2(row_scale, row_scale), base2 = f2(base, base);
           uint64_t sum2[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
@@ -800,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
         if (rec) {
-          rec[128 * kRows] = m;
+          rec[128 * kRows] = m - weight_lift;  // what O and l are relative to
           rec[129 * kRows] = l;
         }
       }
@@ -960,7 +975,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             v_top = max(v_top, octave_top<kHalf>(top));
             v_low = min(v_low, octave_low(low));
             v_small = __any_sync(0xffffffffu, v_low < 0x387fu);
-            if (!wide && !fp16_holds<kHalf>(v_low, v_top)) u.wide = 1;
+            if (!wide && v_top != 0) {
+              const uint32_t mine = octave(v_top) | octave(v_low + 1u);
+              const uint32_t all = atomicOr(&u.v_octaves[c], mine) | mine;
+              if (!fp16_holds<kHalf>(v_low, v_top) || 32 - __clz(all) - __ffs(all) > kApart)
+                u.wide = 1;
+            }
           }
         } else if (__any_sync(0xffffffffu, top > k_top || low < k_low)) {
           // past the end slots hold anything, and a scale that is no number spoils its

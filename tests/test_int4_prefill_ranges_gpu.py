@@ -114,6 +114,24 @@ def test_one_key_beyond_fp16(cuda_device, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("apart", [12, 16, 20, 26])
+def test_one_token_above_the_others_with_a_low_score(cuda_device, dtype, apart):
+    # its weight is some 2^-apart of the largest one's, its values 2^apart times theirs
+    if dtype == torch.float16 and apart > 24:
+        pytest.skip("values beyond the type")
+    c = Case([20], [400], 4, 1, 16, dtype, seed=apart)
+    key, value = torch.zeros_like(c.key).double(), c.value.double() * 2.0 ** (2 - apart / 2)
+    c.q[:] = c.q[:1, :1].clone()  # one query for all rows and heads
+    direction = c.q[0, 0].double() / c.q[0, 0].double().square().sum() / c.scale
+    key[30] = -apart * np.log(2.0) * direction
+    value[30] *= 2.0 ** apart
+    key[31] = 4 * direction  # the row's largest weight, without a value
+    value[31] = 0
+    _rewrite(c, key, value)
+    _check(c, cuda_device, wide=apart > 18)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("exponents", [(0, 8, -8, 0), (-14, 0, 0, 12), (0, 40, -40, 0)])
 def test_groups_far_apart(cuda_device, dtype, exponents):
     if dtype == torch.float16 and max(exponents) > 15:
