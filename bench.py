@@ -42,11 +42,14 @@ import torch
 REPO = Path(__file__).resolve().parent
 if str(REPO) not in sys.path:
     sys.path.insert(0, str(REPO))
-from baseline import install_ref  # noqa: E402
+from baseline import install_ref, stand_in  # noqa: E402
 
 # The engine this backend plugs into (nanovllm), installed unmodified into
 # baseline/_ref, and the reference's test helpers the reference arm times.
 ENGINE_INSTALLED = install_ref.add_to_path()
+# Without the engine the backend runs on a stand-in for its contract, and the
+# records' config says so.
+STAND_IN = stand_in.add()
 METRIC = "paged decode attn+KV-append HBM GB/s and tokens/s at 1/2/4/8 B200"
 TOTAL_Q_HEADS, TOTAL_KV_HEADS, HEAD_DIM, BLOCK_SIZE = 32, 8, 128, 16
 BATCH, CONTEXT = 256, 4096
@@ -670,6 +673,8 @@ def run_ours(args, rank, world, local_rank):
             "timed_loop": "the K steps (append + attention each) captured as one CUDA graph "
                           "and replayed once (full-decode graph path); the decode launch timed "
                           "separately for the roofline",
+            "engine": ("a stand-in for its backend contract (not installed)" if STAND_IN
+                       else "nanovllm from baseline/_ref"),
         },
         "tokens_per_s": round(args.batch / (ms_per_step * 1e-3), 1),
         "bytes_per_step": total_bytes,

@@ -5,7 +5,8 @@ The backend in this package is a plugin of the Nano-vLLM-v1 engine
 the engine's ``AttentionPlan``, registers in the engine's
 ``AttentionBackendRegistry`` and validates metadata with the engine's own
 validator. There is no copy of those classes here, so the engine must be
-importable wherever the backend is used:
+importable wherever the backend is used (the tests, ``smoke()`` and ``bench.py``
+put ``baseline.stand_in`` in this module's place where it is not):
 
 * ``BatchType``, ``CommonAttentionMetadata`` — nanovllm/utils/context.py:7-44
 * ``AttentionRoute``, ``AttentionPlan`` — nanovllm/layers/attention_backend.py:112-135
