@@ -12,9 +12,13 @@
 // neighbouring 256-byte pieces of the same rows, and tokens in consecutive
 // slots write consecutive bytes of the head-major page. More tokens a thread,
 // with their loads issued together, were no faster (2: the same, 4: 72 us);
-// the read-back slows down with them (59 us, 68, 83). What bounds both is DRAM,
-// and with scattered slots the 8-byte scales, which cost a 32-byte sector each
-// (128k tokens of 8 heads: 113 us in order, 145 us in random order).
+// the read-back slows down with them (59 us, 68, 83). What bounds both is DRAM.
+// 128k tokens of 8 heads, us of the append and of the read-back: slots in order 111
+// and 110, whole pages in random order 113 and 112 (6.1 TB/s, 0.93 of the measured
+// rate), slots in random order 148 and 149 (4.6 TB/s); the size of the pages, 16 to
+// 256, changes each by 3 % at most. At random slots the counters show 16 % and 2 % more
+// traffic than the algorithm's (8-byte scales in 32-byte sectors), which is not the
+// third that they cost; pieces of 64 and of 8 bytes are all that is consecutive there.
 #include <cuda_runtime.h>
 
 #include "common.cuh"

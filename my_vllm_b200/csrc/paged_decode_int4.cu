@@ -29,8 +29,8 @@
 // lengths: a share is a run of segments, each the whole of a (sequence, KV
 // head) or a part of it. Parts are joined by a second kernel. (One CTA per
 // partition of a sequence left SMs idle in the last wave and waited 3 to 4 us at
-// its start: 4 x 32768 tokens of 8 KV heads 44.5 us, now 34.9; one head of 512
-// rows of 1024 to 8192 tokens 86.6 us, now 77.4.) Short sequences that one wave of
+// its start: 4 x 32768 tokens of 8 KV heads 44.5 us against 34.9, one head of 512
+// rows of 1024 to 8192 tokens 86.6 us against 77.4, at the time.) Short sequences that one wave of
 // CTAs takes whole are not cut and not joined. The 4 warps take a quarter of a
 // segment each, with its own ring of two stages (2 KiB of K codes, 2 KiB of V
 // codes, 256 bytes of K and of V scales) that it fills itself with 16-byte
@@ -43,13 +43,18 @@
 // units that read the same tiles. A K row's 16-byte chunk and a V chunk's 8 columns
 // of 16 bits are both one scale group.
 //
-// What bounds it is instruction issue, not HBM: a warp spends 464 instructions on
-// a tile of 4608 bytes (of these 221 on the ALU pipe at two cycles each, 34 MMAs at
-// eight), so an SM needs 110 to 140 ns a tile where its share of HBM brings one in
-// 104 ns. 256 x 4096 tokens, 32/8 heads: 205 to 215 us, 5.6 to 5.9 TB/s of 6.5
-// measured; 64 x 4096: 61.6 us, 4.9 TB/s. Tried and not kept: four CTAs per SM
-// (registers spill: 70 against 65 us), a third stage (64.4 against 61.6), e4m3
-// operands for K (their MMAs are taken apart into fp16 ones: 69).
+// What bounds it is the chain of a tile, not HBM and no single pipe: time times the
+// SM clock stays the same while the clock varies (256 x 4096 tokens, 32/8 heads: 215 to
+// 218 us at 1965 MHz, 240 at 1732 under the power cap, 242 cycles a tile and SM both
+// times), so memory does not set the pace, at 0.77 to 0.86 of its measured rate; and
+// of the issue slots 54 % are used, of the MMA pipe 30 %. A warp spends 487
+// instructions on a tile of 4608 bytes (231 of them on the ALU pipe), and with three
+// warps a scheduler 4.7 cycles pass between two of a warp's: 1.1 on fixed latencies, 0.7
+// not chosen, 0.7 on memory, 0.6 on busy pipes, 0.3 on shared memory. 64 x 4096: 63.4 us,
+// 4.8 TB/s; one head of 512 rows 82.9 us, 4.1 TB/s (both 1965 MHz; 581 instructions a
+// tile with 8 heads). Tried and not kept: four CTAs per SM (registers spill: 70 against
+// 65 us), a third stage (64.4 against 61.6), e4m3 operands for K (their MMAs are taken
+// apart into fp16 ones: 69).
 #include <cuda_runtime.h>
 #include <math.h>
 
@@ -87,8 +92,11 @@ constexpr int kPlaceUnit = 128;
 constexpr uint32_t kNoPlace = 0xffffffffu;
 // A CTA takes at least so many tiles: fewer, and joining the parts costs more.
 constexpr int kMinTiles = 4;
-// Sequences of up to so many tiles are not cut where one wave of CTAs holds them
-// (8 sequences of 1 to 512 tokens, 8 KV heads: 7.6 us, cut 10.1).
+// Sequences of up to so many tiles are not cut where one wave of CTAs holds them.
+// us, whole and cut, with 16/8 heads: 1 x 512 tokens 6.0 and 7.6, 1 x 1024 8.3 and 7.8,
+// 1 x 2048 12.8 and 8.7; 24 x 512 7.7 and 13.5, 24 x 1024 11.0 and 15.8, 24 x 2048 18.7
+// and 20.6; 55 x 1 to 2048 21 and 44. So one sequence could go whole to 768 tokens, and
+// many to 2048 and past it; the edge stands where whole is the faster for all.
 constexpr int kWholeTiles = 16;
 
 // Weights of a (head, group) may grow past kMostWeight before their power of two is

@@ -7,12 +7,15 @@
 //
 // Bound: the MMAs (4 x 128 operations per row and token) and, right behind
 // them, an exp2 per row and token; the cache is 3.6 times smaller than in 16
-// bits and never bounds. What does is the instructions of turning codes into
-// operands: 3 to 4 per pair of values next to the softmax's 7 per pair of
-// scores, on the same four schedulers, which issue about one every other cycle.
-// So both are kept short, and their loops small: at 14 KB of hot code more than
-// a third of the fetches missed the instruction cache (1.8 ms for the first case
-// below, 1.3 once they were short).
+// bits and never bounds. What does is a tile's chain: S, its softmax and PV of a Q
+// tile follow one another, as P lies over S, and one softmax warp a scheduler and Q
+// tile walks through it. 2048 rows on 8k tokens: the MMA pipe is 40 % active, 52 % of
+// the issue slots are used, and of the 7.2 cycles between two instructions of a warp
+// 2.0 wait for tensor memory and barriers, 1.7 for fixed latencies, 0.9 for
+// instructions. The converters' instructions (3 to 4 per pair of values next to the
+// softmax's 7 per pair of scores) are in that chain's way, so both are kept short, and
+// their loops small: at 14 KB of hot code more than a third of the fetches missed the
+// instruction cache (1.8 ms for 2048 rows on 32k tokens, 1.3 once they were short).
 //
 // Work. A unit is (sequence, block of 256 packed rows, KV head): the (token, q
 // head of the group) rows of 256 / group query tokens, two UMMA M = 128 tiles A
@@ -27,10 +30,14 @@
 //     the workspace and are joined in part order by a second kernel; a cut within
 //     kMinPart tiles of a unit's end moves there. Without a workspace cuts move to
 //     the nearest end.
-// Measured (32 q heads, 8 KV heads, bf16; us): 2048 rows on 32k tokens, 256 equal
-// units on 148 SMs, whole 1370, cut 1060 (1.01 PFLOP/s); 64 rows on 8k, 8 units,
-// 191 and 46; four chunks of 512 on 512 to 2560 tokens, 76 and 97; two prompts of
-// 2048, 119 and 141; one of 8192, 622 and 736.
+// Measured (32 q heads, 8 KV heads, bf16; us, whole and cut): 2048 rows on 32k tokens,
+// 256 equal units on 148 SMs, 1280 and 1241 (1204 in short runs: 0.89 PFLOP/s); on 8k,
+// 307 and 300; 64 rows on 8k, 8 units, 170 and 45, eight of them 176 and 104; four
+// chunks of 512 on 512 to 2560 tokens, 76 and 97; two prompts of 2048, 120 and 138; one
+// of 8192, 684 and 734. The rule looks at the longest unit and the share only and not
+// at how whole units fall on the SMs, so near its edges it can take the slower: three
+// chunks of 512 on 512 to 2560 tokens 67 and 80, and cut; a prompt of 4096 184 and 214,
+// cut; 19 x 64 rows on 2048 tokens, 152 equal units, 106 and 82, and whole.
 //
 // A CTA's 16 warps:
 //   0-3, 4-7  softmax of tile A, B: thread = row = TMEM lane. A row's 128 scores
