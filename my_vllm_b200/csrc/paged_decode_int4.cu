@@ -692,8 +692,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            float next = fmaxf(base[c], floorf(m));
-            if (next == kNegInf) next = 0.f;
+            // (scores of -inf alone leave it below every score)
+            const float next = fmaxf(fmaxf(base[c], floorf(m)), -3.4e38f);
             up[c] = most < 0.f ? 0 : static_cast<int>(fminf(next - base[c], 512.f));
             base[c] = next;
             l_run[c] *= pow2(-up[c]);
@@ -831,7 +831,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
         auto total = [&](const float (&x)[4], int i) {
           return kBlocks == 1 ? x[2 * i] + x[2 * i + 1] : x[2 * i + c];
         };
-        const float own = 1.f / l_run[c];  // the warp's own result, which stays in range
+        // the warp's own result, which stays in range; scores of -inf alone have none
+        const float own = l_run[c] == 0.f ? 0.f : 1.f / l_run[c];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           float mine, other;
@@ -871,7 +872,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtasPerSm)
         l += f[w];
       }
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      const float inv = 1.f / l;
+      // a part with scores of -inf alone is nothing; a whole sequence of them has no result
+      const float inv = l == 0.f && !whole ? 0.f : 1.f / l;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         if (ml[w * 2 * kHeads + head] == kNegInf) continue;
@@ -934,7 +936,7 @@ __global__ void __launch_bounds__(kWarps * 32) int4_join_kernel(const Int4Decode
   if (!empty) parts = __ldcg(p.parts + (int64_t)b * p.num_units + kvh * p.splits + half);
   const int n = parts.z;
   if (!empty && n == 0) return;  // the whole of it is in place
-  float m = -INFINITY, l = 0.f;
+  float m = -3.4e38f, l = 0.f;  // (a part with scores of -inf alone has -inf)
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   constexpr int kAtOnce = 4;  // parts in flight per warp
   for (int i0 = warp; i0 < n; i0 += kWarps * kAtOnce) {

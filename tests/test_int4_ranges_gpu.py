@@ -177,3 +177,19 @@ def test_small_softmax_scales(cuda_device, scale):
     c.q[0] *= 2.0 ** -10
     c.scale = scale
     _check(c, cuda_device)
+
+
+@pytest.mark.parametrize("parts", [1, 3])
+@pytest.mark.parametrize("hq,hkv", [(4, 1), (8, 1)])
+def test_scores_of_minus_infinity_in_front(cuda_device, hq, hkv, parts):
+    # scores below fp32's range against the first 13 pages, and some -3000 behind them
+    c = Case([1], [500], hq, hkv, 16, torch.bfloat16, seed=5)
+    key = c.key.double() + _push(c, 0, 0, [-400.0] * hq)
+    key[:208] = _push(c, 0, 0, [-1.0] * hq) * 2.0 ** 126
+    _rewrite(c, key)
+    c.scale *= 8
+    out = _decode(c, cuda_device, parts)
+    # as if those pages were not there
+    ref, bounds = int4.attention(c.q.double().numpy(), c.k.numpy(), c.v.numpy(),
+                                 c.tables.numpy()[:, 13:], [292], [0, 1], c.scale)
+    assert_within(out, ref, decode_tolerance(ref, bounds, c.dtype))
