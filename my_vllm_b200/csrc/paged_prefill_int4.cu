@@ -64,14 +64,14 @@
 // rounded to the operands' type while l sums it unrounded.
 //
 // A unit with a scale that fp16 does not hold is run a second time, before the CTA's
-// next units; its first results are overwritten. Keys are then multiplied by a power
-// of two that brings the unit's largest scale to 2^13 at most, and stay exact but for
-// what lies 2^25 and more below it; weights and values are bf16 (2^-8 each). fp16
+// next units; its first results are overwritten. Weights and values are bf16 then (2^-8
+// each). Keys stay exact in fp16, times a power of two of the unit, while their scales
+// lie within 2^25; beyond that they, and the queries, are bf16 as well. fp16
 // calls need it as well: the cache has no type, and a value that overflows is 0 times
 // infinity in every row that does not see it. A converter warp looks closer where a
-// scale lies outside the octaves that it has met in the unit, so this costs two votes
-// and 20 instructions an item (chunks of 512 on 0 to 2048 tokens: 75.6 us without the
-// fp16 calls' run, 76.2 with it).
+// scale lies outside the octaves that it has met in the unit, so this costs a vote and
+// some ten instructions an item (chunks of 512 on 0 to 2048 tokens: 75.6 us without it,
+// 76.6 with it).
 #include <cuda_runtime.h>
 #include <math.h>
 
@@ -117,8 +117,10 @@ struct Unit {
   int lim[2];    // tiles that A, B need: [0, lim)
   int rec;       // record of a part, or -1: the whole unit
   int nan[4];    // first token whose value group g has no finite scale
-  int wide;      // 0, 1 when a scale is found that fp16 operands do not hold, 2 the second run
-  uint32_t k_top;         // largest key scale, bf16 bits
+  // 0, 1 when a scale is found that fp16 operands do not hold; the second run: 2 with
+  // weights and values in bf16, 3 with keys and queries as well
+  int wide;
+  uint32_t k_ranges;      // of the key scales, the ends: bit i from 2^(5 i - 80) on, 0 and 31 also beyond
   uint32_t v_octaves[4];  // of value group g's scales, the ends: bit i from 2^(i - 18) on, 0 also below
 };
 
@@ -296,7 +298,7 @@ __device__ void put_unit(const Int4PrefillParams& p, Unit& u, const SeqInfo& q, 
   u.lim[1] = rows > kRows ? tiles : 0;
   u.rec = t0 > 0 ? 2 * (int)blockIdx.x : t1 < tiles ? 2 * (int)blockIdx.x + 1 : -1;
   u.wide = 0;
-  u.k_top = 0;
+  u.k_ranges = 0;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     u.nan[g] = 0x7fffffff;
@@ -369,6 +371,18 @@ __device__ void list_units(const Int4PrefillParams& p, Shared* sh, bool first) {
   sh->tiles = total;
 }
 
+// Key scales by fives of octaves. Where six of them hold all keys of a unit, a power of
+// two brings its scales to [2^-17, 2^13), where fp16 holds s (c - 8) exactly.
+__device__ __forceinline__ uint32_t key_range(uint32_t bits) {
+  return 1u << min(max((static_cast<int>(bits >> 7) - 47) / 5, 0), 31);
+}
+__device__ __forceinline__ bool keys_shifted(uint32_t ranges) {
+  return 32 - __clz(ranges) - __ffs(ranges) <= 5 && !(ranges & 0x80000001u);
+}
+__device__ __forceinline__ int key_shift(uint32_t ranges) {  // its exponent
+  return ranges == 0 ? 0 : 88 - 5 * (31 - __clz(ranges));
+}
+
 // The units of the list that have to run again; true if there are any.
 __device__ bool list_wide(Shared* sh) {
   int n = 0, total = 0;
@@ -376,7 +390,7 @@ __device__ bool list_wide(Shared* sh) {
     if (sh->units[e].wide != 1) continue;
     Unit& u = sh->units[n++];
     u = sh->units[e];
-    u.wide = 2;
+    u.wide = keys_shifted(u.k_ranges) ? 2 : 3;
 #pragma unroll
     for (int g = 0; g < 4; ++g) u.nan[g] = 0x7fffffff;
     total += u.t1 - u.t0;
@@ -422,7 +436,8 @@ struct ConvertBf16 {
   }
 };
 // fp16: both nibbles of a byte fit the mantissa, 1024 + c and 1024 + 16 c, and one
-// add or fma makes either c - 8. kSmall: scales below 2^-14, subnormal in fp16, are
+// add or fma makes either c - 8 (the published way of turning small integers into
+// floating point: as the low bits of a number whose last place is 1). kSmall: scales below 2^-14, subnormal in fp16, are
 // multiplied in as 256 s, exact down to 2^-22, and the last product, by 2^-8, rounds.
 template <bool kSmall>
 struct ConvertHalf {
@@ -479,11 +494,6 @@ __device__ __forceinline__ uint32_t octave_top(uint32_t bits) {
 __device__ __forceinline__ uint32_t octave_low(uint32_t less_one) {
   return ((less_one + 1u) & ~0x7fu) - 1u;
 }
-// What key scales are multiplied with in a second run, from the largest: to below 2^13.
-__device__ __forceinline__ int key_shift(uint32_t k_top) {
-  return k_top == 0 ? 0 : 139 - static_cast<int>(k_top >> 7);
-}
-
 // One lane's 32 codes -> four 16-byte chunks at shared addresses dst[j] + kOff.
 template <int kOff, typename C>
 __device__ __forceinline__ void convert32(const C& f, const uint4& w, const uint32_t (&dst)[4]) {
@@ -619,13 +629,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     float scale = p.scale_log2;  // of this thread's row in the unit whose Q is ordered
     auto order_q = [&](int e) {
       asm volatile("cp.async.wait_all;" ::: "memory");
-      const bool wide = sh->units[e].wide == 2;
+      const int wide = sh->units[e].wide;
       int shift = 0;
 #pragma unroll 2
       for (int i = 0; i < 32; i += 2) {
         uint4* ptr = reinterpret_cast<uint4*>(qtile + (qc >> 3) * kHalfBytes + swz128(qr + i, qc & 7));
         uint4 v = *ptr;
-        if (!kHalf) {
+        if (kHalf && wide == 3) {
+          auto brain = [&](uint32_t w) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+            return Elem<__nv_bfloat16>::pack(f.x, f.y);
+          };
+          v = make_uint4(brain(v.x), brain(v.y), brain(v.z), brain(v.w));
+        }
+        if (!kHalf && wide != 3) {
           uint32_t most = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
                                    __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
           most = max(most & 0xffffu, most >> 16);
@@ -645,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         *ptr = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
                           __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
       }
-      if (wide) shift += key_shift(sh->units[e].k_top);
+      if (wide == 2) shift += key_shift(sh->units[e].k_ranges);
       // never 0: masked scores are -inf, and stay so
       scale = fmaxf(ldexpf(p.scale_log2, -shift), 1.1754944e-38f);
       fence_proxy_async_smem();
@@ -672,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int seen = min(qpos + 1, u.seq_len);  // tokens this row sees
         float m = -INFINITY, l = 0.f;
         const float row_scale = scale;
-        const bool wide = u.wide == 2;
+        const bool wide = u.wide >= 2;
         const float weight_lift = wide ? -kRescale : kWeightLift;
         for (int j = t0; j < end; ++j) {
           const bool got = mbar_wait(smem_u32(&sh->s_full[x]), done & 1);
@@ -950,7 +967,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const bool more = next.e >= 0;
         Unit& u = sh->units[now.e];
-        const bool wide = u.wide == 2;
+        const int wide = u.wide;
         if (met != now.e) {
           met = now.e;
           k_top = v_top = 0;
@@ -982,7 +999,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             v_top = max(v_top, octave_top<kHalf>(top));
             v_low = min(v_low, octave_low(low));
             v_small = __any_sync(0xffffffffu, v_low < 0x387fu);
-            if (!wide && v_top != 0) {
+            if (wide < 2 && v_top != 0) {
               const uint32_t mine = octave(v_top) | octave(v_low + 1u);
               const uint32_t all = atomicOr(&u.v_octaves[c], mine) | mine;
               if (!fp16_holds<kHalf>(v_low, v_top) || 32 - __clz(all) - __ffs(all) > kApart)
@@ -998,14 +1015,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               k_top = max(k_top, octave_top<kHalf>(bits[k]));
               k_low = min(k_low, octave_low(bits[k] - 1u));
             }
-          // of all groups and rows: the smallest keys only count if all are small
           k_top = __reduce_max_sync(0xffffffffu, k_top);
           k_low = __reduce_min_sync(0xffffffffu, k_low);
           k_small = k_low < 0x387fu;
-          if (!wide) {
-            k_top = max(k_top, atomicMax(&u.k_top, k_top));
-            if (!fp16_holds<kHalf>(k_low, k_top) ||
-                (kHalf && k_top < 0x3b00u && k_low < 0x36ffu))  // 2^-9, 2^-17
+          if (wide < 2 && k_top != 0) {
+            const uint32_t mine = key_range(k_top) | key_range(k_low + 1u);
+            const uint32_t all = atomicOr(&u.k_ranges, mine) | mine;
+            // fp16 calls: keys below 2^-17 only count if all are below 2^-10
+            if (!fp16_holds<kHalf>(k_low, k_top) || (kHalf && k_low < 0x36ffu && all < 1u << 14))
               u.wide = 1;
           }
         }
@@ -1019,11 +1036,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           row8(std::integral_constant<int, 2>());
           row8(std::integral_constant<int, 3>());
         };
-        if (wide) {
-          if (now.is_v) {
+        if (wide >= 2) {
+          if (now.is_v || wide == 3) {
             rows([](uint32_t b) { return ConvertBf16(b); });
           } else {
-            const int shift = key_shift(u.k_top);
+            const int shift = key_shift(u.k_ranges);
             const float f0 = ldexpf(1.f, shift / 2), f1 = ldexpf(1.f, shift - shift / 2);
             rows([&](uint32_t b) { return ConvertHalf<true>(__uint_as_float(b << 16) * f0 * f1); });
           }
@@ -1049,8 +1066,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------------------------------------------------------- MMAs --
-    // S in fp16; PV in bf16 in a second run
-    const uint32_t idesc_s = f16_instr_desc(kRows, kTokens, false, false);
     int pv0 = 0, pv1 = 0, qn0 = 0, qn1 = 0;  // tiles and units issued per Q tile
     int tiles = 0;
     while (true) {
@@ -1059,6 +1074,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int n_tiles = sh->tiles;
       if (elect_one()) {
         bool ok = true;
+        uint32_t idesc_s = 0;  // of the unit that S is in
         // n = -1 only begins tile 0's S
         Cursor cur, nxt;
         nxt.seek(sh);
@@ -1077,7 +1093,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const Unit& u = sh->units[cur.e];
               const uint64_t vd = smem_desc(sbase + kV0 + (g & 1) * kTileBytes, kHalfBytes, 1024);
               const uint32_t par = (x ? pv1 : pv0) & 1;
-              const uint32_t idesc_pv = f16_instr_desc(kRows, kHeadDim, u.wide == 2, true);
+              const uint32_t idesc_pv = f16_instr_desc(kRows, kHeadDim, u.wide >= 2, true);
               ok = mbar_wait(smem_u32(&sh->p_lo[x]), par) &&
                    mbar_wait(smem_u32(&sh->v_full[g & 1]), (g >> 1) & 1);
               if (!ok) break;
@@ -1098,6 +1114,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (more && nxt.t < sh->units[nxt.e].lim[x]) {  // S of tile g + 1
               if (nxt.t == sh->units[nxt.e].t0) {
+                idesc_s = f16_instr_desc(kRows, kTokens, sh->units[nxt.e].wide == 3, false);
                 ok = mbar_wait(smem_u32(&sh->q_full[x]), (x ? qn1 : qn0) & 1);
                 if (!ok) break;
                 if (x) ++qn1; else ++qn0;

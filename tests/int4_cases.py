@@ -83,16 +83,19 @@ def assert_within(out, ref, tol):
         f"allowed, at {np.unravel_index(over.argmax(), over.shape)}")
 
 
-def prefill_bound(ref, bounds, dtype, wide=False):
+def prefill_bound(ref, bounds, dtype, wide=False, bf16_keys=False):
     """The bound of prefill by the operands that a unit really runs with. fp16: keys and
     values are exact and weights round by 2^-11 (those below 2^-21 of a row's largest
     round to multiples of 2^-32 of it: that, for values whose scales lie up to 2^18
     apart, is within the 2^-19 that covers the exponentials). ``wide``: weights and
-    values in bf16, keys still exact. Scores stay in fp32 as in decode. fp16 outputs
-    below its normal range are off by half their step, 2^-25."""
+    values in bf16, keys still exact; ``bf16_keys``: keys, and the queries of fp16 calls, in
+    bf16 too. Scores stay in fp32 as in decode. fp16 outputs below its normal range are off
+    by half their step, 2^-25."""
     bf16 = UNIT[torch.bfloat16]
     rounded = 2 * bf16 + bf16 ** 2 if wide else UNIT[torch.float16]
-    weight = rounded + 2.0 ** -19 + np.expm1(2 * 2.0 ** -19 * bounds["terms"])[..., None]
+    operands = (2 * bf16 + bf16 ** 2 if dtype == torch.float16 else bf16) if bf16_keys else 0.0
+    score = operands * bounds["keys"] + 2.0 ** -19 * bounds["terms"]
+    weight = rounded + 2.0 ** -19 + np.expm1(2 * score)[..., None]
     u = UNIT[dtype]
     least = 2.0 ** -25 if dtype == torch.float16 else 1e-37
     return u * np.abs(ref) + weight * bounds["mass"] * (1 + u) + least

@@ -103,6 +103,29 @@ def test_keys_beyond_fp16(cuda_device, dtype, factor):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("apart", [20, 30, 40, 90, 120])
+@pytest.mark.parametrize("q,kv", [(20, 400), (20, 3000)])
+def test_a_key_far_above_the_others_that_no_row_wants(cuda_device, dtype, apart, q, kv):
+    # its scores are far below every other, whose keys it must not cost anything
+    c = Case([q], [kv], 4, 1, 16, dtype, seed=apart)
+    c.q[:] = c.q[:1, :1].clone()
+    direction = c.q[0, 0].double() / c.q[0, 0].double().square().sum() / c.scale
+    key = c.key.double()
+    key[30] = -direction * 2.0 ** apart
+    _rewrite(c, key, dtype=torch.bfloat16)
+    out = _prefill(c, cuda_device)
+    # the same with a key that is just low enough, and the bound of the keys that count
+    key[30] = -200 * direction
+    _rewrite(c, key, dtype=torch.bfloat16)
+    ref, bounds = c.reference()
+    key[30] = 0
+    _rewrite(c, key, dtype=torch.bfloat16)
+    others = c.reference()[1]
+    bounds.update(keys=others["keys"], terms=others["terms"])
+    assert_within(out, ref, prefill_bound(ref, bounds, dtype, wide=True, bf16_keys=True))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_one_key_beyond_fp16(cuda_device, dtype):
     # scores of 2^14 and more against one token; rows that see it give it everything, or nothing
     c = Case([40], [300], 4, 1, 16, dtype, seed=7)
